@@ -53,6 +53,15 @@ SIGNATURES = {
     "dsa_topk_select": [P, I64, P, P, I64, I64, I64, P, P, INT, P],
     "dsa_indexer_topk": [P, P, I64, P, I64, P, P, I64, P, I64, I64, I64, I64, I64, I64, P, P, P,
                          INT, P, P],
+    "dsa_step_layout": [P, P, I64, P, I64, I64, P, I64, P, I64, P, P, P, P, P, P, P],
+    "dsa_apply_rope": [P, I64, I64, P, I64, I64, INT, I64, I64, I64, I64, I64, P, INT, P, INT, INT, F32,
+                       P],
+    "dsa_latent_cache_append": [P, I64, INT, P, INT, I64, P, INT, P, P, P, I64, I64, P, I64, I64, I64,
+                                F32, INT, F32, P, P],
+    "dsa_shared_prefix_attention_workspace_size": [I64, I64, ctypes.POINTER(SZ)],
+    "dsa_shared_prefix_attention": [P, I64, I64, P, I64, I64, P, I64, I64, P, I64, I64, P, I64, P, P, I64,
+                                    I64, I64, P, P, I64, I64, I64, F32, P, I64, I64, P, I64, I64, P, SZ,
+                                    P],
 }
 
 
@@ -96,3 +105,21 @@ def check(fn_name: str, rc: int):
 
 def call(fn_name: str, *args):
     check(fn_name, getattr(load(), fn_name)(*args))
+
+
+def call_on(device, fn_name: str, *args):
+    """`call` with `device` current and torch's current stream of that device
+    as the last argument."""
+    import torch
+    if device.index is None or device.index == torch.cuda.current_device():
+        check(fn_name, getattr(load(), fn_name)(*args, torch.cuda.current_stream(device).cuda_stream))
+    else:
+        with torch.cuda.device(device):
+            check(fn_name, getattr(load(), fn_name)(*args, torch.cuda.current_stream(device).cuda_stream))
+
+
+def check_cuda(device, **tensors):
+    """RuntimeError unless every tensor (None is skipped) is on the CUDA `device`."""
+    for name, t in tensors.items():
+        if t is not None and (not t.is_cuda or t.device != device):
+            raise RuntimeError(f"{name} must be a CUDA tensor on {device} (no CPU path), got {t.device}")

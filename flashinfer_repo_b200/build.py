@@ -2,7 +2,7 @@
 
     python -m flashinfer_repo_b200.build [--force]
 
-Compiles every csrc/*.cu with nvcc for sm_100a only, links the CUDA runtime
+Compiles every csrc/*.cu and csrc/step/*.cu with nvcc for sm_100a only, links the CUDA runtime
 statically (so the library loads on machines without a driver, e.g. for the
 symbol checks) and writes flashinfer_repo_b200/libdsa_b200.so.
 """
@@ -37,7 +37,7 @@ def nvcc() -> str:
 
 
 def sources():
-    return sorted(glob.glob(os.path.join(CSRC, "*.cu")))
+    return sorted(glob.glob(os.path.join(CSRC, "*.cu")) + glob.glob(os.path.join(CSRC, "step", "*.cu")))
 
 
 def _stale(target, deps):
@@ -49,7 +49,8 @@ def _stale(target, deps):
 
 def build(force: bool = False, verbose: bool = False) -> str:
     os.makedirs(BUILD_DIR, exist_ok=True)
-    headers = glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(INCLUDE, "*.h"))
+    headers = (glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(CSRC, "step", "*.cuh")) +
+               glob.glob(os.path.join(INCLUDE, "*.h")))
     objs = []
     procs = []
     for src in sources():

@@ -13,6 +13,7 @@ namespace dsa {
 enum : int {
   kErrBadIndex = 1,     // an index outside [-1, num_slots)
   kErrTimeout = 2,      // a bounded mbarrier wait gave up
+  kErrCapacity = 4,     // more pages or rows wanted than there is room for
 };
 
 // ~2 s at 2 GHz: far beyond any legitimate wait in these kernels.

@@ -1,0 +1,133 @@
+// latent_append.cu -- writes new rows of the paged latent cache: the 512-wide
+// latent normalised and weighted, the 64-wide rotary key turned to its position,
+//   ckv[slot] = bf16(x * rsqrt(mean(x^2) + eps) * w),  kpe[slot] = bf16(turn(x[512:576])).
+// Sums and products in 32 bits, one rounding at the store.
+//
+// One warp per row: 16 latent values and one rotary pair a lane, the sum of
+// squares by shuffles, one angle a lane.  Bound by HBM for a prefill batch
+// (1152 bytes in and out a row) and by latency for a decode step.
+#include "../../../include/dsa_b200.h"
+#include "rotate.cuh"
+
+namespace dsa {
+namespace {
+
+constexpr int kLatent = 512, kRot = 64;
+
+struct AppendParams {
+  const void* kv;
+  int64_t kv_st;
+  const void* w;
+  int w_dtype;
+  int64_t rows;
+  const void* positions;
+  int pos64;
+  const int32_t* slots;
+  const double* inv_freq;
+  __nv_bfloat16 *ckv, *kpe;
+  int64_t ckv_sp, ckv_sr, kpe_sp, kpe_sr, num_pages;
+  float eps, scale;
+  int half_layout;
+  int* err;
+};
+
+__device__ __forceinline__ float weight(const AppendParams& p, int i) {
+  if (p.w_dtype == DSA_FP32) return static_cast<const float*>(p.w)[i];
+  if (p.w_dtype == DSA_FP16) return to_f32(static_cast<const __half*>(p.w)[i]);
+  return to_f32(static_cast<const __nv_bfloat16*>(p.w)[i]);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) dsa_latent_append_kernel(const AppendParams p) {
+  const int64_t row = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+  const int lane = threadIdx.x & 31;
+  if (row >= p.rows) return;
+  const int32_t slot = p.slots[row];
+  if (slot < 0) {  // a padded row; anything below -1 is a wrong id
+    if (slot < -1 && lane == 0) set_error(p.err, kErrBadIndex);
+    return;
+  }
+  const int64_t page = slot >> 6, at = slot & 63;
+  if (page >= p.num_pages) {
+    if (lane == 0) set_error(p.err, kErrBadIndex);
+    return;
+  }
+  const T* x = static_cast<const T*>(p.kv) + row * p.kv_st;
+  float v[16], sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    v[k] = to_f32(x[(k >> 3) * 256 + lane * 8 + (k & 7)]);
+    sum += v[k] * v[k];
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  const float r = 1.f / sqrtf(sum * (1.f / kLatent) + p.eps);
+  __nv_bfloat16* c = p.ckv + page * p.ckv_sp + at * p.ckv_sr;
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    const int i = (k >> 3) * 256 + lane * 8 + (k & 7);
+    c[i] = __float2bfloat16_rn(v[k] * r * weight(p, i));
+  }
+  const int ia = p.half_layout ? lane : 2 * lane, ib = p.half_layout ? lane + 32 : 2 * lane + 1;
+  const float a = to_f32(x[kLatent + ia]), b = to_f32(x[kLatent + ib]);
+  float cs, sn;
+  rotation(load_position(p.positions, p.pos64, row), p.inv_freq[lane], p.scale, &cs, &sn);
+  __nv_bfloat16* e = p.kpe + page * p.kpe_sp + at * p.kpe_sr;
+  e[ia] = __float2bfloat16_rn(a * cs - b * sn);
+  e[ib] = __float2bfloat16_rn(b * cs + a * sn);
+}
+
+}  // namespace
+}  // namespace dsa
+
+using namespace dsa;
+
+extern "C" int dsa_latent_cache_append(const void* kv, int64_t kv_stride, int kv_dtype, const void* norm_weight,
+                                       int norm_dtype, int64_t num_tokens, const void* positions,
+                                       int positions_are_64_bit, const int32_t* slots, const double* inv_freq,
+                                       void* ckv_cache, int64_t ckv_stride_page, int64_t ckv_stride_row,
+                                       void* kpe_cache, int64_t kpe_stride_page, int64_t kpe_stride_row,
+                                       int64_t num_pages, float eps, int layout, float rope_scale,
+                                       int* device_error, void* stream) {
+  if (num_tokens < 0 || num_pages < 0) return report_error(DSA_ERR_INVALID_ARG, "negative size");
+  if (layout != DSA_ROPE_INTERLEAVED && layout != DSA_ROPE_HALF)
+    return report_error(DSA_ERR_INVALID_ARG, "unknown rotary layout");
+  for (int t : {kv_dtype, norm_dtype})
+    if (t != DSA_BF16 && t != DSA_FP16 && t != DSA_FP32)
+      return report_error(DSA_ERR_INVALID_ARG, "unknown element type");
+  if (num_tokens == 0) return DSA_OK;
+  if (!kv || !norm_weight || !positions || !slots || !inv_freq || !ckv_cache || !kpe_cache)
+    return report_error(DSA_ERR_INVALID_ARG, "NULL pointer argument");
+  AppendParams p;
+  p.kv = kv;
+  p.kv_st = kv_stride;
+  p.w = norm_weight;
+  p.w_dtype = norm_dtype;
+  p.rows = num_tokens;
+  p.positions = positions;
+  p.pos64 = positions_are_64_bit != 0;
+  p.slots = slots;
+  p.inv_freq = inv_freq;
+  p.ckv = static_cast<__nv_bfloat16*>(ckv_cache);
+  p.kpe = static_cast<__nv_bfloat16*>(kpe_cache);
+  p.ckv_sp = ckv_stride_page;
+  p.ckv_sr = ckv_stride_row;
+  p.kpe_sp = kpe_stride_page;
+  p.kpe_sr = kpe_stride_row;
+  p.num_pages = num_pages;
+  p.eps = eps;
+  p.scale = rope_scale;
+  p.half_layout = layout == DSA_ROPE_HALF;
+  p.err = device_error;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const unsigned grid = (unsigned)((num_tokens * 32 + 255) / 256);
+  if (kv_dtype == DSA_BF16)
+    dsa_latent_append_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(p);
+  else if (kv_dtype == DSA_FP16)
+    dsa_latent_append_kernel<__half><<<grid, 256, 0, s>>>(p);
+  else
+    dsa_latent_append_kernel<float><<<grid, 256, 0, s>>>(p);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return report_error(DSA_ERR_CUDA, cudaGetErrorString(e));
+  return DSA_OK;
+}

@@ -11,6 +11,10 @@ i.e. it assumes one query per KV token.  Here:
     decode token per request, token b <-> request b);
   * nothing synchronises with the host, so the whole step can be captured in
     a CUDA graph (`DecodeStepGraph`).
+
+`run_shared_prefix_step` is the dense counterpart for requests behind one shared
+prefix: lay the step out -> write the latent cache -> rotate the queries ->
+attention over the prefix and the requests' own rows.
 """
 from __future__ import annotations
 
@@ -18,6 +22,10 @@ import torch
 
 from . import indexer as IX
 from .kernel import kernel
+from .latent_cache import latent_cache_append
+from .layout import step_layout
+from .prefix import shared_prefix_attention
+from .rope import apply_rope
 
 
 def run_sparse_attention_pipeline(q_index_fp8, k_index_cache_fp8, k_scale, weights, seq_lens,
@@ -35,6 +43,28 @@ def run_sparse_attention_pipeline(q_index_fp8, k_index_cache_fp8, k_scale, weigh
     out, lse = kernel(q_nope, q_pe, ckv_cache, kpe_cache, sparse_indices, sm_scale, output=output,
                       lse=lse)
     return out, lse, slots
+
+
+def run_shared_prefix_step(q_nope, q_pe, kv, norm_weight, inv_freq, ckv_cache, kpe_cache, seq_lens,
+                           query_lens, block_table, free_pages, prefix_pages, prefix_len, sm_scale, *,
+                           rope_layout="interleaved", rope_scale=1.0, eps=1e-6, output=None, lse=None,
+                           device_error=None, workspace=None):
+    """One step of requests that share a prefix: q_nope [T,H,512], q_pe [T,H,64]
+    (not rotated) and kv [T,576] hold the new tokens in request order, request b
+    has query_lens[b] of them on top of seq_lens[b] own rows in the cache.
+    prefix_len is a [1] int32 tensor.  block_table is extended in place with
+    pages of free_pages.  Nothing synchronises with the host.  Returns (output,
+    lse, layout); rows behind the last request's attend to the prefix only."""
+    lay = step_layout(seq_lens, query_lens, block_table, free_pages, q_nope.shape[0], prefix_len=prefix_len,
+                      device_error=device_error)
+    latent_cache_append(kv, norm_weight, lay.positions, lay.slots, inv_freq, ckv_cache, kpe_cache, eps=eps,
+                        layout=rope_layout, rope_scale=rope_scale, device_error=device_error)
+    q_pe = apply_rope(q_pe, lay.positions, inv_freq, layout=rope_layout, scale=rope_scale)
+    out, lse = shared_prefix_attention(q_nope, q_pe, ckv_cache, kpe_cache, prefix_pages, prefix_len,
+                                       block_table, lay.token_lens, sm_scale,
+                                       token_request=lay.token_request, output=output, lse=lse,
+                                       workspace=workspace)
+    return out, lse, lay
 
 
 class DecodeStepGraph:

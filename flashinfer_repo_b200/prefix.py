@@ -1,0 +1,144 @@
+"""Dense MLA attention over the paged latent cache for a batch that shares a
+long prefix: the prefix's rows are read once for all the tokens.
+
+Stands beside `kernel()`, which attends to 2048 selected rows of the same cache:
+this one attends to every row of the shared prefix and of the request's own
+pages (short contexts, exact attention behind a common system prompt or
+document).  The reference has no counterpart.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+from .kernel import HEAD_DIM_CKV, HEAD_DIM_KPE, NUM_HEADS, PAGE_SIZE, _rowmajor
+
+_workspaces: dict[int, list] = {}  # per device: every buffer handed out, the newest last
+_size_cache: dict[tuple, int] = {}
+
+
+def prefix_workspace_size(num_tokens: int, heads: int = NUM_HEADS, device=None) -> int:
+    """Bytes of the workspace that a call of this shape needs on `device`
+    (default: the current device)."""
+    device = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    nbytes = _size_cache.get((index, num_tokens, heads))
+    if nbytes is None:
+        n = ctypes.c_size_t(0)
+        with torch.cuda.device(index):
+            _lib.call("dsa_shared_prefix_attention_workspace_size", num_tokens, heads, ctypes.byref(n))
+        nbytes = _size_cache[(index, num_tokens, heads)] = n.value
+    return nbytes
+
+
+def _workspace(device, nbytes):
+    """The device's shared workspace.  A larger call gets a new buffer; older
+    ones are kept, since a captured graph may hold their address."""
+    kept = _workspaces.setdefault(device.index, [])
+    if not kept or kept[-1].numel() < nbytes:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the workspace must grow during stream capture: make one call of this size before "
+                               "the capture, or pass workspace=")
+        kept.append(torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device))
+    return kept[-1]
+
+
+def shared_prefix_attention(q_nope, q_pe, ckv_cache, kpe_cache, prefix_pages, prefix_len, block_table, token_lens,
+                            sm_scale, *, token_request=None, output=None, lse=None, workspace=None):
+    """Attention of every token over the shared prefix and its request's own rows;
+    returns (output [T,H,512] bf16, lse [T,H] fp32 base 2).
+
+    q_nope [T,H,512], q_pe [T,H,64], ckv_cache [P,64,512], kpe_cache [P,64,64]
+    bf16, H a multiple of 16.  prefix_pages [n] int32 and prefix_len (an int or
+    a [1] int32 CUDA tensor, at most 64 n): the prefix, which may end inside a
+    page.  block_table [B,W] int32: own pages of each request, own row 0 first.
+    token_lens [T] int32: own rows that token t sees (0: only the prefix).
+    token_request [T] int32: block-table row of token t (default: row t).
+    `step_layout` makes token_lens and token_request.  A token that sees no row
+    gets output 0 and lse -inf.  Rows past a length are never read.
+
+    output/lse write into existing tensors.  workspace: a zeroed uint8 CUDA
+    tensor of prefix_workspace_size(T, H) bytes for calls that may run at the
+    same time as others on the device (the default one is shared, so such calls
+    must not overlap).  Errors found on the device (page ids or requests outside
+    their range: those rows are skipped) are read by `read_prefix_error`.
+    """
+    tokens, heads, dim = q_nope.shape
+    num_pages = ckv_cache.shape[0]
+    assert heads % NUM_HEADS == 0 and heads > 0, "heads must be a multiple of 16"
+    assert dim == HEAD_DIM_CKV and q_pe.shape == (tokens, heads, HEAD_DIM_KPE)
+    assert ckv_cache.shape == (num_pages, PAGE_SIZE, HEAD_DIM_CKV)
+    assert kpe_cache.shape == (num_pages, PAGE_SIZE, HEAD_DIM_KPE)
+    assert block_table.dim() == 2 and prefix_pages.dim() == 1 and token_lens.shape == (tokens,)
+    device = q_nope.device
+    length = prefix_len if isinstance(prefix_len, torch.Tensor) else None
+    _lib.check_cuda(device, q_nope=q_nope, q_pe=q_pe, ckv_cache=ckv_cache, kpe_cache=kpe_cache,
+                    prefix_pages=prefix_pages, prefix_len=length, block_table=block_table, token_lens=token_lens,
+                    token_request=token_request, output=output, lse=lse)
+    for name, t in (("q_nope", q_nope), ("q_pe", q_pe), ("ckv_cache", ckv_cache), ("kpe_cache", kpe_cache)):
+        assert t.dtype == torch.bfloat16, f"{name} must be bfloat16"
+    for name, t in (("prefix_pages", prefix_pages), ("block_table", block_table), ("token_lens", token_lens)):
+        assert t.dtype in (torch.int32, torch.int64), f"{name} must be int32 or int64"
+    if length is not None:
+        assert length.numel() == 1 and length.dtype == torch.int32, "prefix_len must be an int or one int32"
+        bound = prefix_pages.shape[0] * PAGE_SIZE
+    else:
+        bound = int(prefix_len)
+        assert 0 <= bound <= prefix_pages.shape[0] * PAGE_SIZE, "prefix_len does not fit prefix_pages"
+    if token_request is not None:
+        assert token_request.shape == (tokens,) and token_request.dtype in (torch.int32, torch.int64)
+        token_request = _int32(token_request)
+    else:
+        assert block_table.shape[0] >= tokens, "without token_request the block table needs a row for every token"
+    if output is None:
+        output = torch.empty((tokens, heads, HEAD_DIM_CKV), dtype=torch.bfloat16, device=device)
+    else:
+        assert output.shape == (tokens, heads, HEAD_DIM_CKV) and output.dtype == torch.bfloat16
+        assert output.stride(-1) == 1 and output.stride(0) % 8 == 0 and output.stride(1) % 8 == 0 \
+            and output.data_ptr() % 16 == 0, "output rows must be contiguous and 16-byte aligned"
+    if lse is None:
+        lse = torch.empty((tokens, heads), dtype=torch.float32, device=device)
+    else:
+        assert lse.shape == (tokens, heads) and lse.dtype == torch.float32
+    if tokens == 0:
+        return output, lse
+    prefix_pages, token_lens = _int32(prefix_pages), _int32(token_lens)
+    if block_table.dtype != torch.int32 or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        block_table = block_table.to(torch.int32).contiguous()
+    q_nope, q_pe = _rowmajor(q_nope, 8), _rowmajor(q_pe, 8)
+    ckv_cache, kpe_cache = _rowmajor(ckv_cache, 8), _rowmajor(kpe_cache, 8)
+    if workspace is None:
+        workspace = _workspace(device, prefix_workspace_size(tokens, heads, device))
+    elif not (workspace.is_cuda and workspace.device == device and workspace.dtype == torch.uint8
+              and workspace.is_contiguous()):
+        raise ValueError("workspace must be a contiguous uint8 tensor on the inputs' device")
+    _lib.call_on(device, "dsa_shared_prefix_attention", q_nope.data_ptr(), q_nope.stride(0), q_nope.stride(1),
+                 q_pe.data_ptr(), q_pe.stride(0), q_pe.stride(1), ckv_cache.data_ptr(), ckv_cache.stride(0),
+                 ckv_cache.stride(1), kpe_cache.data_ptr(), kpe_cache.stride(0), kpe_cache.stride(1),
+                 prefix_pages.data_ptr(), bound, length.data_ptr() if length is not None else None,
+                 block_table.data_ptr(), block_table.stride(0), block_table.shape[0], block_table.shape[1],
+                 token_request.data_ptr() if token_request is not None else None, token_lens.data_ptr(), tokens,
+                 heads, num_pages, float(sm_scale), output.data_ptr(), output.stride(0), output.stride(1),
+                 lse.data_ptr(), lse.stride(0), lse.stride(1), workspace.data_ptr(), workspace.numel())
+    return output, lse
+
+
+def _int32(t: torch.Tensor) -> torch.Tensor:
+    return t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
+
+
+def read_prefix_error(device=None, clear=True) -> int:
+    """Synchronise and return the DSA_DEVERR_* bits raised by
+    shared_prefix_attention calls that used the device's shared workspace."""
+    device = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    bits = 0
+    with torch.cuda.device(index):
+        stream = torch.cuda.current_stream().cuda_stream
+        for buf in _workspaces.get(index, []):
+            word = ctypes.c_int(0)
+            _lib.call("dsa_read_device_error", buf.data_ptr(), int(clear), ctypes.byref(word), stream)
+            bits |= word.value
+    return bits

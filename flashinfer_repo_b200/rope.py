@@ -1,0 +1,100 @@
+"""Rotary positions for queries and keys of the DSA step.
+
+The reference takes rotated q_pe, k_pe and index queries (solution/triton/
+kernel.py:138, indexer_kernel.py:345) and has no operator that makes them.
+Angles are position * inv_freq with inv_freq in 64 bits, reduced on the device
+before they are rounded, so far positions lose nothing and there is no table of
+cosines to size or gather.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _lib
+
+LAYOUTS = {"interleaved": 0, "half": 1}
+DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def rope_frequencies(rot_dim, base=10000.0, *, scaling=None, factor=1.0, original_context=4096, beta_fast=32.0,
+                     beta_slow=1.0, device="cuda") -> torch.Tensor:
+    """inv_freq [rot_dim/2] float64 = base^(-2i/rot_dim), stretched for long contexts:
+
+    scaling None      as they are
+    "linear"          every frequency divided by `factor`
+    "ntk"             the base grows, base * factor^(rot_dim/(rot_dim-2))
+    "yarn"            by parts: pairs that turn more than beta_fast times over
+                      original_context stay, those under beta_slow turns are
+                      divided by `factor`, a linear ramp between
+    """
+    rot_dim = int(rot_dim)
+    assert rot_dim >= 2 and rot_dim % 2 == 0, "rot_dim must be even"
+    if scaling not in (None, "linear", "ntk", "yarn"):
+        raise ValueError(f"unknown scaling {scaling!r}")
+    if scaling is not None and not factor >= 1.0:
+        raise ValueError("factor must be at least 1")
+    if scaling == "ntk":
+        assert rot_dim > 2, "ntk scaling needs more than one pair"
+        base = base * factor ** (rot_dim / (rot_dim - 2))
+    i = torch.arange(0, rot_dim, 2, dtype=torch.float64)
+    inv = base ** (-i / rot_dim)
+    if scaling == "linear":
+        inv = inv / factor
+    elif scaling == "yarn":
+        def pair(turns):  # the (fractional) pair that makes `turns` turns over the original context
+            return rot_dim * math.log(original_context / (turns * 2 * math.pi)) / (2 * math.log(base))
+        low, high = max(math.floor(pair(beta_fast)), 0), min(math.ceil(pair(beta_slow)), rot_dim - 1)
+        ramp = ((torch.arange(rot_dim // 2, dtype=torch.float64) - low) / max(high - low, 1e-3)).clamp(0, 1)
+        inv = inv * (1 - ramp) + inv / factor * ramp
+    return inv.to(device)
+
+
+def _check_rotation(device, positions, inv_freq, tokens, layout):
+    if layout not in LAYOUTS:
+        raise ValueError(f"layout must be one of {sorted(LAYOUTS)}, got {layout!r}")
+    assert positions.shape == (tokens,) and positions.dtype in (torch.int32, torch.int64), \
+        "positions must be [tokens] int32 or int64"
+    assert inv_freq.dim() == 1 and inv_freq.dtype == torch.float64, "inv_freq must be [rot_dim/2] float64"
+    _lib.check_cuda(device, positions=positions, inv_freq=inv_freq)
+    return positions.contiguous(), inv_freq.contiguous()
+
+
+def apply_rope(x, positions, inv_freq, *, layout="interleaved", offset=0, inverse=False, scale=1.0, out=None):
+    """Turn the slice [offset, offset + rot_dim) of every head of x [T, H, D]
+    (or [T, D]) to its token's position, rot_dim = 2 * len(inv_freq); the other
+    values are copied.
+
+    positions [T] int32 or int64; inv_freq float64 (`rope_frequencies`).
+    layout "interleaved" pairs values (2i, 2i+1) of the slice, "half" (i, i +
+    rot_dim/2).  scale multiplies the turned slice (the attention factor of
+    scaled frequencies).  inverse=True turns back: with the same scale it is the
+    gradient of the forward turn.  out: a tensor of x's shape and type to write
+    into, x itself for in place; any other overlap with x is not allowed.
+    bf16, fp16 or fp32; products in 32 bits, one rounding.
+    """
+    assert x.dim() in (2, 3), "x must be [tokens, heads, dim] or [tokens, dim]"
+    assert x.dtype in DTYPES, f"x must be bf16, fp16 or fp32, got {x.dtype}"
+    device, tokens = x.device, x.shape[0]
+    _lib.check_cuda(device, x=x, out=out)
+    positions, inv_freq = _check_rotation(device, positions, inv_freq, tokens, layout)
+    rot = 2 * inv_freq.shape[0]
+    assert 0 <= offset and offset + rot <= x.shape[-1], "the rotated slice reaches past the head"
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=device)
+        if x.stride(-1) != 1:
+            x = x.contiguous()
+    else:
+        assert out.shape == x.shape and out.dtype == x.dtype and out.stride(-1) == 1
+        if x.stride(-1) != 1:
+            assert out.data_ptr() != x.data_ptr()
+            x = x.contiguous()
+        if out.data_ptr() == x.data_ptr():
+            assert out.stride() == x.stride(), "out shares x's memory with other strides"
+    heads = x.shape[1] if x.dim() == 3 else 1
+    _lib.call_on(device, "dsa_apply_rope", x.data_ptr(), x.stride(0), x.stride(-2) if x.dim() == 3 else 0,
+                 out.data_ptr(), out.stride(0), out.stride(-2) if x.dim() == 3 else 0, DTYPES[x.dtype], tokens,
+                 heads, x.shape[-1], int(offset), rot, positions.data_ptr(), int(positions.dtype == torch.int64),
+                 inv_freq.data_ptr(), LAYOUTS[layout], int(bool(inverse)), float(scale))
+    return out

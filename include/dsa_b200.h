@@ -43,7 +43,17 @@ enum dsa_status {
 /* Bits of the device error word (first int of a workspace). */
 enum dsa_device_error {
   DSA_DEVERR_BAD_INDEX = 1, /* an index outside [-1, num_pages*64): row skipped */
-  DSA_DEVERR_TIMEOUT = 2    /* a bounded wait inside a kernel gave up */
+  DSA_DEVERR_TIMEOUT = 2,   /* a bounded wait inside a kernel gave up */
+  DSA_DEVERR_CAPACITY = 4   /* dsa_step_layout: out of free pages, table columns or rows */
+};
+
+/* Element types of the operators that take more than one. */
+enum dsa_dtype { DSA_BF16 = 0, DSA_FP16 = 1, DSA_FP32 = 2 };
+
+/* Which values of a rotated slice of width r form pair i. */
+enum dsa_rope_layout {
+  DSA_ROPE_INTERLEAVED = 0, /* (2i, 2i + 1) */
+  DSA_ROPE_HALF = 1         /* (i, i + r/2) */
 };
 
 /* Message of the last failing call on this host thread ("" if none). */
@@ -307,6 +317,107 @@ int dsa_index_cache_append(const void* keys_bf16, int64_t num_tokens, const int3
                            void* k_cache_fp8, int64_t k_page_stride, void* k_scale,
                            int64_t scale_page_stride, int64_t num_pages, int* device_error,
                            void* stream);
+
+/*
+ * Where the new rows of a step go.  Request b has seq_lens[b] rows in the cache
+ * and gets query_lens[b] more (both int32 on the device; negative counts as 0).
+ * block_table [batch, max_pages] is extended in place: entries
+ * [ceil(s/64), ceil((s+q)/64)) of row b take the next pages of free_pages, in
+ * request order from its front; every other entry is left as it was.  Row i of
+ * the outputs (int32, num_tokens rows) is the i-th new row in request order:
+ *   slots          table[b][pos/64]*64 + pos%64 with pos = s + j, what
+ *                  dsa_index_cache_append and dsa_latent_cache_append take
+ *   positions      *prefix_len + pos (prefix_len: one int32 on the device, or
+ *                  NULL for 0: the shared prefix in front of every request)
+ *   token_request  b
+ *   token_lens     pos + 1: the own rows that this token sees
+ * Rows behind the last request get slot -1, position 0, request 0, length 0.
+ * *pages_used receives how many free pages were taken.  Running the same step
+ * again writes the same values.  Where free pages, table columns or output rows
+ * run out, the rows concerned get slot -1 (table entry -1) or are dropped and
+ * DSA_DEVERR_CAPACITY is set; a negative entry of an older page gives slot -1
+ * and DSA_DEVERR_BAD_INDEX.  device_error may be NULL.  No counterpart in the
+ * reference, whose caller builds these on the host.
+ */
+int dsa_step_layout(const int32_t* seq_lens, const int32_t* query_lens, int64_t batch,
+                    int32_t* block_table, int64_t block_table_stride, int64_t max_pages,
+                    const int32_t* free_pages, int64_t num_free, const int32_t* prefix_len,
+                    int64_t num_tokens, int32_t* slots, int32_t* positions, int32_t* token_request,
+                    int32_t* token_lens, int32_t* pages_used, int* device_error, void* stream);
+
+/*
+ * Rotary positions: out = x [num_tokens, num_heads, head_dim] with the slice
+ * [rot_offset, rot_offset + rot_dim) of every head turned,
+ *   (a, b) -> scale * (a cos - b sin, b cos + a sin),
+ * angle = positions[token] * inv_freq[i] for pair i (inv_freq: rot_dim/2 fp64
+ * values on the device; the angle is reduced in 64 bits, the products are in 32).
+ * inverse != 0 turns back, which with the same scale is also the gradient.
+ * Strides are in elements, the last dimension is contiguous; out may be x (then
+ * only the slice is written) but must not overlap it in another way.  rot_dim is
+ * even, at most 512.  positions are int32 or int64.  No counterpart in the
+ * reference, which takes rotated queries and keys.
+ */
+int dsa_apply_rope(const void* x, int64_t x_stride_token, int64_t x_stride_head, void* out,
+                   int64_t out_stride_token, int64_t out_stride_head, int dtype, int64_t num_tokens,
+                   int64_t num_heads, int64_t head_dim, int64_t rot_offset, int64_t rot_dim,
+                   const void* positions, int positions_are_64_bit, const double* inv_freq, int layout,
+                   int inverse, float scale, void* stream);
+
+/*
+ * New rows of the paged latent cache that dsa_sparse_attention and
+ * dsa_shared_prefix_attention read.  Row i of kv [num_tokens, 576] goes to slot
+ * slots[i] (page*64 + row; -1 = skip):
+ *   ckv row = bf16(x[0:512] * rsqrt(mean(x[0:512]^2) + eps) * norm_weight)
+ *   kpe row = bf16(rope_scale * x[512:576] turned to positions[i])
+ * kv and norm_weight [512] are bf16, fp16 or fp32 (dsa_dtype); inv_freq holds 32
+ * fp64 values.  Strides in elements.  Slots must be distinct.  A slot past the
+ * last page (or below -1) is skipped and sets DSA_DEVERR_BAD_INDEX.  No
+ * counterpart in the reference, which takes a filled cache.
+ */
+int dsa_latent_cache_append(const void* kv, int64_t kv_stride, int kv_dtype, const void* norm_weight,
+                            int norm_dtype, int64_t num_tokens, const void* positions,
+                            int positions_are_64_bit, const int32_t* slots, const double* inv_freq,
+                            void* ckv_cache, int64_t ckv_stride_page, int64_t ckv_stride_row,
+                            void* kpe_cache, int64_t kpe_stride_page, int64_t kpe_stride_row,
+                            int64_t num_pages, float eps, int layout, float rope_scale,
+                            int* device_error, void* stream);
+
+/* Workspace bytes dsa_shared_prefix_attention needs for this shape on the
+ * current device (the device error word in the first 256 bytes, then the launch
+ * plan and the partial results of row blocks that several CTAs share). */
+int dsa_shared_prefix_attention_workspace_size(int64_t num_tokens, int64_t num_heads, size_t* bytes);
+
+/*
+ * Dense MLA attention for a batch whose requests share one prefix: token t
+ * attends to the prefix's rows and to the first token_lens[t] rows of its
+ * request's own pages.
+ *   q_nope [T, H, 512], q_pe [T, H, 64], ckv [P, 64, 512], kpe [P, 64, 64] bf16
+ *   prefix_pages   int32, ceil(max_prefix_len/64) page ids of the prefix
+ *   prefix_len     one int32 on the device (at most max_prefix_len), or NULL
+ *                  for max_prefix_len; the prefix may end inside a page
+ *   block_table    [batch, max_pages] int32: own pages, own row 0 first
+ *   token_request  [T] int32 row of the block table, or NULL: token t has row t
+ *   token_lens     [T] int32, own rows that the token sees (0 allowed)
+ *   output [T, H, 512] bf16, lse [T, H] fp32 (base 2); a token that sees nothing
+ *   gets output 0 and lse -inf
+ * H is a multiple of 16.  Strides in elements, last dimensions contiguous; query
+ * and cache rows 16-byte aligned, output rows 16-byte aligned.  Lengths are read
+ * on the device, so a captured call follows them.  Cache rows past a length are
+ * never read.  A page id outside [0, num_pages), a request outside [0, batch) or
+ * a length past the table is skipped and sets DSA_DEVERR_BAD_INDEX in the
+ * workspace's first word.  The workspace follows dsa_sparse_attention's rules.
+ * No counterpart in the reference.
+ */
+int dsa_shared_prefix_attention(
+    const void* q_nope, int64_t q_nope_stride_token, int64_t q_nope_stride_head, const void* q_pe,
+    int64_t q_pe_stride_token, int64_t q_pe_stride_head, const void* ckv_cache, int64_t ckv_stride_page,
+    int64_t ckv_stride_row, const void* kpe_cache, int64_t kpe_stride_page, int64_t kpe_stride_row,
+    const int32_t* prefix_pages, int64_t max_prefix_len, const int32_t* prefix_len,
+    const int32_t* block_table, int64_t block_table_stride, int64_t batch, int64_t max_pages,
+    const int32_t* token_request, const int32_t* token_lens, int64_t num_tokens, int64_t num_heads,
+    int64_t num_pages, float sm_scale, void* output, int64_t out_stride_token, int64_t out_stride_head,
+    float* lse, int64_t lse_stride_token, int64_t lse_stride_head, void* workspace,
+    size_t workspace_bytes, void* stream);
 
 /*
  * Read (and optionally clear) the device error word of a workspace.
