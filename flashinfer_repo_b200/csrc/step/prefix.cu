@@ -3,127 +3,768 @@
 // the first token_lens[t] rows of its request's own pages,
 //   o = sum_k p_k ckv_k / sum_k p_k,  p_k = exp(sm_scale (q_nope.ckv_k + q_pe.kpe_k)),
 //   lse = log2 sum_k p_k.
-// One pass over the rows with the running maximum and sum of the softmax.
+//
+// Every token reads the same prefix rows, so the (token, head) rows of the whole
+// batch are stacked and a row block of 128 of them (8 tokens of 16 heads, or one
+// of 128) meets each cache row once: 2 * 128 * 1088 operations a cache row of 1152
+// bytes, work for the 5th-generation tensor cores.  An accumulator of 128 rows x
+// 512 values alone fills a CTA's tensor memory, so a PAIR of CTAs shares a row
+// block (tcgen05 cta_group::2, M = 128): each holds 64 of its rows, O takes 256
+// TMEM columns and two buffers of scores 64 each.  A tile is two cache pages
+// (128 rows): CTA c stages page c for Q.K^T (N = 128 from the pair) and its 256
+// of the 512 values of both pages for P.V (N = 256 from the pair).
+//
+// The pages of a row block form one list -- the prefix, then the own pages of its
+// tokens one after the other -- and the lists of all row blocks are cut evenly
+// over the pairs (one persistent cluster per two SMs); a row block that several
+// pairs share is joined by a merge grid.  A token's own page is masked for the
+// other tokens of the block twice: their weights are not counted, and the MMA
+// leaves their TMEM lanes alone, so a request whose rows hold NaN or infinities
+// cannot touch another's output.  Rows behind a length are never read: a partly
+// filled page is loaded from a row coordinate below zero, which moves its rows to
+// the end of the tile and has the TMA write zeros before them.
+#include <cuda.h>
+
+#include <mutex>
+
 #include "../../../include/dsa_b200.h"
-#include "../common.cuh"
+#include "pair.cuh"
 
 namespace dsa {
 namespace {
 
-constexpr int kPreThreads = 256;
-constexpr int kRowPitch = 584;  // 576 values and 16 bytes: rows start in different banks
+constexpr int kRows = 64;                      // (token, head) rows per CTA
+constexpr int kGroups = 8;                     // 16-head groups per row block
+constexpr int kPanel = 64 * 128;               // 64 rows x 64 values, 128-byte swizzle
+constexpr int kKChunk = 3 * kPanel;            // a third of the 576 key values of a page
+constexpr int kVChunk = 4 * kPanel;            // 128 values of both pages
+constexpr int kThreads = 12 * 32;
+constexpr int kSoftmaxThreads = 256;
+constexpr uint32_t kTmemS = 256;               // TMEM columns: O 0-255, scores 256 and 320
+constexpr int kSlotFloats = 2 * kRows * 512 + 4 * kRows;  // partial: O, m, l of 128 rows
+constexpr int kPlanThreads = 1024;
+constexpr float kLazy = 8.f;  // the running maximum follows only a rise of more than 2^8
 
 struct PrefixParams {
-  const __nv_bfloat16 *qn, *qp, *ckv, *kpe;
-  int64_t qn_st, qn_sh, qp_st, qp_sh, ckv_sp, ckv_sr, kpe_sp, kpe_sr;
   const int32_t *prefix_pages, *prefix_len, *block_table, *token_request, *token_lens;
-  int64_t max_prefix, bt_stride, batch, max_pages, tokens, num_pages;
-  int heads;
+  int64_t max_prefix, bt_stride, batch, max_pages, tokens, num_pages, groups, blocks;
+  int group_per_token, max_pairs;
   float scale_log2;
   __nv_bfloat16* out;
   int64_t out_st, out_sh;
   float* lse;
   int64_t lse_st, lse_sh;
   int* err;
+  long long* cum;  // [blocks + 1] tiles before each row block
+  float* parts;    // [blocks + max_pairs] partials
 };
 
-struct PreSmem {
-  __nv_bfloat16 kv[64][kRowPitch];
-  __nv_bfloat16 q[16][kRowPitch];
-  float s[16][64];
-  float m[16], l[16], alpha[16];
+__device__ __forceinline__ int64_t prefix_rows(const PrefixParams& p) {
+  return p.prefix_len ? min(p.max_prefix, (int64_t)max(*p.prefix_len, 0)) : p.max_prefix;
+}
+// Own rows of token t and its row of the block table; what does not fit the
+// table is cut off.
+__device__ __forceinline__ int64_t own_rows(const PrefixParams& p, int64_t t, int64_t* request, bool* bad) {
+  const int64_t len = max(p.token_lens[t], 0), r = p.token_request ? p.token_request[t] : t;
+  *request = r;
+  if (len == 0) return 0;
+  const bool known = r >= 0 && r < p.batch;
+  *bad = !known || len > p.max_pages * 64;
+  return known ? min(len, p.max_pages * 64) : 0;
+}
+__device__ __forceinline__ int64_t first_token(const PrefixParams& p, int64_t block) {
+  return block * kGroups / p.group_per_token;
+}
+__device__ __forceinline__ int tokens_of(const PrefixParams& p, int64_t block) {
+  const int64_t last = min((block + 1) * kGroups, p.groups) - 1;
+  return (int)(last / p.group_per_token - first_token(p, block)) + 1;
+}
+// The pairs that work: one tile each at least.  Tile u of the U tiles belongs
+// to the pair c with start(c) <= u < start(c + 1).
+__device__ __forceinline__ int pairs_used(const PrefixParams& p, long long tiles) {
+  return (int)min((long long)p.max_pairs, tiles);
+}
+__device__ __forceinline__ long long pair_start(long long tiles, int pairs, int c) { return tiles * c / pairs; }
+__device__ __forceinline__ int pair_of(long long tiles, int pairs, long long u) {
+  return (int)(((u + 1) * pairs - 1) / tiles);
+}
+
+// ------------------------------------------------------------------ plan
+// Tiles before every row block, from the lengths: one CTA, a scan.
+__global__ void __launch_bounds__(kPlanThreads) dsa_prefix_plan_kernel(const PrefixParams p) {
+  __shared__ long long sums[kPlanThreads / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t pre = (prefix_rows(p) + 63) >> 6;
+  long long base = 0;
+  for (int64_t b0 = 0; b0 < p.blocks; b0 += kPlanThreads) {
+    const int64_t b = b0 + threadIdx.x;
+    long long n = 0;
+    if (b < p.blocks) {
+      int64_t pages = pre;
+      const int64_t t0 = first_token(p, b);
+      const int nt = tokens_of(p, b);
+      for (int i = 0; i < nt; ++i) {
+        int64_t r;
+        bool bad = false;
+        pages += (own_rows(p, t0 + i, &r, &bad) + 63) >> 6;
+      }
+      n = max((pages + 1) >> 1, (int64_t)1);  // one at least: an empty row block still writes its rows
+    }
+    long long x = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long a = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += a;
+    }
+    if (lane == 31) sums[warp] = x;
+    __syncthreads();
+    long long before = base, all = 0;
+    for (int w = 0; w < kPlanThreads / 32; ++w) {
+      if (w < warp) before += sums[w];
+      all += sums[w];
+    }
+    if (b < p.blocks) p.cum[b] = before + x - n;
+    base += all;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) p.cum[p.blocks] = base;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+// ------------------------------------------------------------ attention
+// One pair's stretch of a row block's pages.
+struct Segment {
+  int64_t block, request[kGroups];
+  long long tile0, tile1;  // within the row block
+  int64_t pre_pages, pre_rows, pages, own_end[kGroups], own_len[kGroups];
+  int tokens, whole;       // whole: no other pair works on the row block
+  uint32_t mask[kGroups][4];  // TMEM lanes that do not belong to token i, 64 rows of each CTA
 };
 
-__global__ void __launch_bounds__(kPreThreads) dsa_prefix_attention_kernel(const PrefixParams p) {
-  extern __shared__ uint8_t raw[];
-  PreSmem& S = *reinterpret_cast<PreSmem*>(raw);
-  const int64_t t = blockIdx.x;
-  const int h0 = blockIdx.y * 16, tid = threadIdx.x;
-  for (int e = tid; e < 16 * 576; e += kPreThreads) {
-    const int h = e / 576, d = e % 576;
-    S.q[h][d] = d < 512 ? p.qn[t * p.qn_st + (h0 + h) * p.qn_sh + d] : p.qp[t * p.qp_st + (h0 + h) * p.qp_sh + d - 512];
+struct PairSmem {
+  uint8_t q[9][kPanel];
+  uint8_t k[3][kKChunk];
+  uint8_t v[2][kVChunk];
+  uint8_t p[2][kPanel];
+  float red[2][4][kRows];
+  Segment seg[2];
+  int valid[4][2];  // rows of the two pages of the last tiles
+  uint64_t q_full, q_empty, k_full[3], k_empty[3], v_full[2], v_empty[2], s_full[2], p_full, pv_done;
+  uint64_t seg_full[2], seg_empty[2];
+  uint32_t tmem;
+};
+static_assert(sizeof(PairSmem) <= 232448, "shared memory of a CTA");
+
+// Own token of page k of the segment's list, -1 for a prefix page.
+__device__ __forceinline__ int page_token(const Segment& g, int64_t k) {
+  if (k < g.pre_pages) return -1;
+  int i = 0;
+  while (i + 1 < g.tokens && k >= g.own_end[i]) ++i;
+  return i;
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    dsa_prefix_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __grid_constant__ CUtensorMap map_qp,
+                                const __grid_constant__ CUtensorMap map_ckv, const __grid_constant__ CUtensorMap map_kpe,
+                                const __grid_constant__ PrefixParams p) {
+  extern __shared__ __align__(1024) uint8_t raw[];
+  PairSmem& S = *reinterpret_cast<PairSmem*>(raw);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = (int)cluster_ctarank(), pair = blockIdx.x >> 1;
+
+  if (threadIdx.x == 0) {
+    mbar_init(&S.q_full, 2);
+    mbar_init(&S.q_empty, 1);
+    for (int i = 0; i < 3; ++i) {
+      mbar_init(&S.k_full[i], 2);
+      mbar_init(&S.k_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&S.v_full[i], 2);
+      mbar_init(&S.v_empty[i], 1);
+      mbar_init(&S.s_full[i], 1);
+      mbar_init(&S.seg_full[i], 1);
+      mbar_init(&S.seg_empty[i], 8 + 2 + (rank == 0));
+    }
+    mbar_init(&S.p_full, 2 * kSoftmaxThreads / 32);
+    mbar_init(&S.pv_done, 1);
+    fence_mbar_init();
   }
-  if (tid < 16) {
-    S.m[tid] = -INFINITY;
-    S.l[tid] = 0.f;
-  }
-  int64_t prefix = p.max_prefix;
-  if (p.prefix_len) prefix = min(prefix, (int64_t)max(*p.prefix_len, 0));
-  int64_t own = max(p.token_lens[t], 0), req = p.token_request ? p.token_request[t] : t;
-  if (own > 0 && (req < 0 || req >= p.batch || own > p.max_pages * 64)) {
-    if (tid == 0) set_error(p.err, kErrBadIndex);
-    own = (req < 0 || req >= p.batch) ? 0 : p.max_pages * 64;
-  }
-  const int64_t pre_pages = (prefix + 63) / 64, pages = pre_pages + (own + 63) / 64;
-  float o[16][2] = {};
-  for (int64_t k = 0; k < pages; ++k) {
-    const bool is_own = k >= pre_pages;
-    const int64_t kk = is_own ? k - pre_pages : k;
-    const int32_t page = is_own ? p.block_table[req * p.bt_stride + kk] : p.prefix_pages[kk];
-    int valid = (int)min((int64_t)64, (is_own ? own : prefix) - kk * 64);
-    if (page < 0 || page >= p.num_pages) {
-      if (tid == 0) set_error(p.err, kErrBadIndex);
-      valid = 0;
-    }
-    __syncthreads();
-    for (int e = tid; e < 64 * 72; e += kPreThreads) {
-      const int r = e / 72, c = e % 72;
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (r < valid)
-        v = c < 64 ? *reinterpret_cast<const uint4*>(p.ckv + page * p.ckv_sp + r * p.ckv_sr + c * 8)
-                   : *reinterpret_cast<const uint4*>(p.kpe + page * p.kpe_sp + r * p.kpe_sr + (c - 64) * 8);
-      *reinterpret_cast<uint4*>(&S.kv[r][c * 8]) = v;
-    }
-    __syncthreads();
-    {
-      const int r = tid & 63, hb = (tid >> 6) * 4;
-      float acc[4] = {};
-      for (int d = 0; d < 576; ++d) {
-        const float kv = __bfloat162float(S.kv[r][d]);
-#pragma unroll
-        for (int h = 0; h < 4; ++h) acc[h] += __bfloat162float(S.q[hb + h][d]) * kv;
-      }
-#pragma unroll
-      for (int h = 0; h < 4; ++h) S.s[hb + h][r] = r < valid ? acc[h] * p.scale_log2 : -INFINITY;
-    }
-    __syncthreads();
-    if (tid < 16) {
-      float top = S.m[tid];
-      for (int r = 0; r < 64; ++r) top = fmaxf(top, S.s[tid][r]);
-      const float a = top == -INFINITY ? 1.f : exp2f(S.m[tid] - top);
-      float l = S.l[tid] * a;
-      for (int r = 0; r < 64; ++r) {
-        const float e = r < valid ? exp2f(S.s[tid][r] - top) : 0.f;
-        S.s[tid][r] = e;
-        l += e;
-      }
-      S.m[tid] = top;
-      S.l[tid] = l;
-      S.alpha[tid] = a;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int h = 0; h < 16; ++h) {
-      o[h][0] *= S.alpha[h];
-      o[h][1] *= S.alpha[h];
-    }
-    for (int r = 0; r < valid; ++r) {
-      const float v0 = __bfloat162float(S.kv[r][2 * tid]), v1 = __bfloat162float(S.kv[r][2 * tid + 1]);
-#pragma unroll
-      for (int h = 0; h < 16; ++h) {
-        o[h][0] += S.s[h][r] * v0;
-        o[h][1] += S.s[h][r] * v1;
-      }
-    }
-  }
+  if (warp == 9) tmem_alloc_pair(&S.tmem, 512);
+  tc_fence_before();
   __syncthreads();
+  cluster_sync_all();  // both CTAs' barriers and TMEM are there
+  tc_fence_after();
+  const uint32_t tmem = S.tmem;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the plan is written
+
+  const long long tiles = p.cum[p.blocks];
+  const int pairs = pairs_used(p, tiles);
+  const long long u0 = pair < pairs ? pair_start(tiles, pairs, pair) : 0;
+  const long long u1 = pair < pairs ? pair_start(tiles, pairs, pair + 1) : 0;
+
+  if (warp == 11) {
+    // ------------------------------------------------------------- segments
+    int64_t block = 0;
+    if (u0 < u1) {
+      int64_t lo = 0, hi = p.blocks;
+      while (hi - lo > 1) {
+        const int64_t mid = (lo + hi) >> 1;
+        if (p.cum[mid] <= u0)
+          lo = mid;
+        else
+          hi = mid;
+      }
+      block = lo;
+    }
+    long long u = u0;
+    for (int n = 0;; ++n) {
+      const int s = n & 1;
+      if (!mbar_wait(&S.seg_empty[s], ((n >> 1) & 1) ^ 1)) {
+        set_error(p.err, kErrTimeout);
+        break;
+      }
+      Segment& g = S.seg[s];
+      if (u >= u1) {  // no more: an empty segment ends the other roles
+        if (lane == 0) {
+          g.tile0 = g.tile1 = 0;
+          mbar_arrive(&S.seg_full[s]);
+        }
+        break;
+      }
+      const long long c0 = p.cum[block], c1 = p.cum[block + 1];
+      const int nt = tokens_of(p, block);
+      const int64_t t0 = first_token(p, block), pre = prefix_rows(p);
+      int64_t len = 0, req = 0, pages = 0;
+      bool bad = false;
+      if (lane < nt) {
+        len = own_rows(p, t0 + lane, &req, &bad);
+        pages = (len + 63) >> 6;
+      }
+      if (bad) set_error(p.err, kErrBadIndex);
 #pragma unroll
-  for (int h = 0; h < 16; ++h) {
-    const float inv = S.l[h] == 0.f ? 0.f : 1.f / S.l[h];
-    *reinterpret_cast<uint32_t*>(p.out + t * p.out_st + (h0 + h) * p.out_sh + 2 * tid) =
-        pack_bf16(o[h][0] * inv, o[h][1] * inv);
+      for (int o = 1; o < kGroups; o <<= 1) {
+        const int64_t a = __shfl_up_sync(0xffffffffu, pages, o);
+        if (lane >= o) pages += a;
+      }
+      const int64_t pre_pages = (pre + 63) >> 6;
+      if (lane < nt) {
+        g.own_end[lane] = pre_pages + pages;
+        g.own_len[lane] = len;
+        g.request[lane] = req;
+        if (lane == nt - 1) g.pages = pre_pages + pages;
+        uint32_t off[4] = {0, 0, 0, 0};
+        for (int i = 0; i < kGroups; ++i) {
+          const int64_t group = block * kGroups + i;
+          // groups behind the last one are nobody's: their lanes may be written
+          if (group < p.groups && group / p.group_per_token != t0 + lane) off[i >> 1] |= 0xffffu << (16 * (i & 1));
+        }
+        for (int i = 0; i < 4; ++i) g.mask[lane][i] = off[i];
+      }
+      if (lane == 0) {
+        g.block = block;
+        g.tile0 = u - c0;
+        g.tile1 = min(u1, c1) - c0;
+        g.pre_pages = pre_pages;
+        g.pre_rows = pre;
+        g.tokens = nt;
+        g.whole = u == c0 && c1 <= u1;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&S.seg_full[s]);
+      u = min(u1, c1);
+      ++block;
+    }
+  } else if (warp == 8 || warp == 10) {
+    // ------------------------------------------------- loads: Q and K, or V
+    if (elect_one()) {
+      const uint32_t q_bar = cluster_map(smem_u32(&S.q_full), 0);
+      const uint32_t k_bar = cluster_map(smem_u32(&S.k_full[0]), 0), v_bar = cluster_map(smem_u32(&S.v_full[0]), 0);
+      const bool keys = warp == 8;
+      bool ok = true;
+      int it = 0;
+      for (int n = 0; ok; ++n) {
+        const Segment& g = S.seg[n & 1];
+        if (!mbar_wait(&S.seg_full[n & 1], (n >> 1) & 1)) {
+          ok = false;
+          break;
+        }
+        if (g.tile0 >= g.tile1) break;
+        if (keys) {
+          if (!mbar_wait(&S.q_empty, (n & 1) ^ 1)) {
+            ok = false;
+            break;
+          }
+          const int64_t first = g.block * kGroups + rank * 4;
+          const int have = (int)max((int64_t)0, min((int64_t)4, p.groups - first));
+          mbar_arrive_expect_tx_at(q_bar, have * 9 * 2048);
+          for (int i = 0; i < have; ++i) {
+            const int64_t t = (first + i) / p.group_per_token;
+            const int h = (int)((first + i) - t * p.group_per_token) * 16;
+            for (int j = 0; j < 8; ++j)
+              tma_load_3d_pair(smem_u32(S.q[j]) + i * 2048, &map_qn, j * 64, h, (int)t, q_bar);
+            tma_load_3d_pair(smem_u32(S.q[8]) + i * 2048, &map_qp, 0, h, (int)t, q_bar);
+          }
+        }
+        for (long long tile = g.tile0; tile < g.tile1 && ok; ++tile, ++it) {
+          int page[2], row[2], valid[2];  // row: coordinate that puts the valid rows at the end
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int64_t k = 2 * tile + i;
+            int id = -1, rows = 0;
+            if (k < g.pages) {
+              const int t = page_token(g, k);
+              const int64_t at = t < 0 ? k : k - (t ? g.own_end[t - 1] : g.pre_pages);
+              id = t < 0 ? p.prefix_pages[at] : p.block_table[g.request[t] * p.bt_stride + at];
+              rows = (int)min((int64_t)64, (t < 0 ? g.pre_rows : g.own_len[t]) - at * 64);
+              if (id < 0 || id >= p.num_pages) {
+                if (keys) set_error(p.err, kErrBadIndex);
+                rows = 0;
+              }
+            }
+            valid[i] = rows;
+            page[i] = rows ? id : 0;
+            row[i] = rows ? rows - 64 : 64;  // 64: nothing of the page, all zeros
+          }
+          const uint32_t parity = (it & 1) ^ 1;
+          if (keys) {
+#pragma unroll
+            for (int c = 0; c < 3; ++c) {
+              if (!mbar_wait(&S.k_empty[c], parity)) {
+                ok = false;
+                break;
+              }
+              if (c == 0) {
+                S.valid[it & 3][0] = valid[0];
+                S.valid[it & 3][1] = valid[1];
+              }
+              mbar_arrive_expect_tx_at(k_bar + 8 * c, kKChunk);
+#pragma unroll
+              for (int b = 0; b < 3; ++b) {
+                const int j = 3 * c + b;
+                if (j < 8)
+                  tma_load_3d_pair(smem_u32(S.k[c]) + b * kPanel, &map_ckv, j * 64, row[rank], page[rank], k_bar + 8 * c);
+                else
+                  tma_load_3d_pair(smem_u32(S.k[c]) + b * kPanel, &map_kpe, 0, row[rank], page[rank], k_bar + 8 * c);
+              }
+            }
+          } else {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              if (!mbar_wait(&S.v_empty[c], parity)) {
+                ok = false;
+                break;
+              }
+              mbar_arrive_expect_tx_at(v_bar + 8 * c, kVChunk);
+#pragma unroll
+              for (int b = 0; b < 4; ++b)  // page b / 2, columns 64 (b % 2) of this CTA's 128
+                tma_load_3d_pair(smem_u32(S.v[c]) + b * kPanel, &map_ckv, c * 256 + rank * 128 + (b & 1) * 64, row[b >> 1],
+                                 page[b >> 1], v_bar + 8 * c);
+            }
+          }
+        }
+        mbar_arrive(&S.seg_empty[n & 1]);
+      }
+      if (!ok) set_error(p.err, kErrTimeout);
+    }
+    __syncwarp();
+  } else if (warp == 9) {
+    // ----------------------------------------------------------- MMA issue
+    if (rank == 0 && elect_one()) {
+      constexpr uint32_t id_qk = umma_idesc(1, 1, 0, 0, 128, 128);
+      constexpr uint32_t id_pv = umma_idesc(1, 1, 0, 1, 128, 256);
+      const uint64_t q_desc = umma_desc(smem_u32(S.q[0]), 16, 1024, kSwizzle128B);
+      const uint64_t k_desc = umma_desc(smem_u32(S.k[0]), 16, 1024, kSwizzle128B);
+      const uint64_t p_desc = umma_desc(smem_u32(S.p[0]), 16, 1024, kSwizzle128B);
+      const uint64_t v_desc = umma_desc(smem_u32(S.v[0]), kPanel, 1024, kSwizzle128B);
+      bool ok = true;
+      int it = 0;               // tiles whose scores are issued
+      uint32_t off[2][4];       // lanes left alone by the two pages of the tile before
+      bool masked = false;
+      auto weigh = [&](int i) -> bool {  // O += P V of tile i
+        if (!mbar_wait_cluster(&S.p_full, i & 1)) return false;
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          if (!mbar_wait_cluster(&S.v_full[c], i & 1)) return false;
+          tc_fence_after();
+#pragma unroll
+          for (int ks = 0; ks < 8; ++ks) {
+            const uint64_t a = p_desc + (((ks >> 2) * kPanel + (ks & 3) * 32) >> 4);
+            const uint64_t b = v_desc + ((c * kVChunk + (ks >> 2) * 2 * kPanel + (ks & 3) * 2048) >> 4);
+            if (masked)
+              umma_f16_pair_masked(tmem + c * 128, a, b, id_pv, off[ks >> 2]);
+            else
+              umma_f16_pair(tmem + c * 128, a, b, id_pv, 1u);
+          }
+          umma_commit_pair(&S.v_empty[c]);
+        }
+        umma_commit_pair(&S.pv_done);
+        return true;
+      };
+      for (int n = 0; ok; ++n) {
+        const Segment& g = S.seg[n & 1];
+        if (!mbar_wait(&S.seg_full[n & 1], (n >> 1) & 1)) {
+          ok = false;
+          break;
+        }
+        // a segment's last P.V does not wait for the next one's queries
+        if (it > 0 && !weigh(it - 1)) {
+          ok = false;
+          break;
+        }
+        if (g.tile0 >= g.tile1) break;
+        if (!mbar_wait_cluster(&S.q_full, n & 1)) {
+          ok = false;
+          break;
+        }
+        for (long long tile = g.tile0; tile < g.tile1 && ok; ++tile, ++it) {
+#pragma unroll
+          for (int c = 0; c < 3; ++c) {
+            if (!mbar_wait_cluster(&S.k_full[c], it & 1)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+#pragma unroll
+            for (int j = 0; j < 12; ++j)
+              umma_f16_pair(tmem + kTmemS + 64 * (it & 1),
+                            q_desc + (((3 * c + (j >> 2)) * kPanel + (j & 3) * 32) >> 4),
+                            k_desc + ((c * kKChunk + (j >> 2) * kPanel + (j & 3) * 32) >> 4), id_qk,
+                            (c > 0 || j > 0) ? 1u : 0u);
+            umma_commit_pair(&S.k_empty[c]);
+          }
+          if (!ok) break;
+          umma_commit_pair(&S.s_full[it & 1]);
+          if (tile + 1 == g.tile1) umma_commit_pair(&S.q_empty);
+          if (tile > g.tile0 && !weigh(it - 1)) {
+            ok = false;
+            break;
+          }
+          masked = false;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int64_t k = 2 * tile + i;
+            const int t = k < g.pages ? page_token(g, k) : -1;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              off[i][w] = t < 0 ? 0u : g.mask[t][w];
+              masked |= off[i][w] != 0;
+            }
+          }
+        }
+        mbar_arrive(&S.seg_empty[n & 1]);
+      }
+      if (!ok) set_error(p.err, kErrTimeout);
+    }
+    __syncwarp();
+  } else {
+    // --------------------------------------------------- softmax, epilogue
+    // Lane quarter q of TMEM: rows 32 (q & 1) + lane against page q >> 1; the
+    // two warps of a quarter take 32 columns (and 128 columns of O) each.
+    const int quarter = warp & 3, half = warp >> 2, page = quarter >> 1;
+    const int row = (quarter & 1) * 32 + lane;
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t p_bar = cluster_map(smem_u32(&S.p_full), 0);
+    bool ok = true;  // a wait that gave up takes all eight warps out at their next barrier
+    int it = 0;
+    for (int n = 0;; ++n) {
+      const Segment& g = S.seg[n & 1];
+      ok = mbar_wait(&S.seg_full[n & 1], (n >> 1) & 1);
+      if (!named_bar_all(1, kSoftmaxThreads, ok)) break;
+      if (g.tile0 >= g.tile1) break;
+      const int64_t group = g.block * kGroups + rank * 4 + (row >> 4);
+      const bool live = group < p.groups;
+      const int64_t token = live ? group / p.group_per_token : 0;
+      const int mine = live ? (int)(token - first_token(p, g.block)) : -2;  // its place in the block
+      float m = -INFINITY, l = 0.f;
+      for (long long tile = g.tile0; tile < g.tile1; ++tile, ++it) {
+        const int64_t k = 2 * tile + page;
+        ok = ok && mbar_wait_cluster(&S.s_full[it & 1], (it >> 1) & 1);
+        tc_fence_after();
+        const int t = k < g.pages ? page_token(g, k) : -1;
+        const bool sees = live && (t < 0 || t == mine);
+        // the page's rows are at the end of its 64 columns
+        const int from = sees ? 64 - S.valid[it & 3][page] - 32 * half : 32;
+        float x[32];
+        tmem_ld32(lanes + kTmemS + 64 * (it & 1) + 32 * half, x);
+        float top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          x[j] = j >= from ? x[j] * p.scale_log2 : -INFINITY;
+          top = fmaxf(top, x[j]);
+        }
+        S.red[it & 1][page * 2 + half][row] = top;
+        if (!(ok = named_bar_all(1, kSoftmaxThreads, ok))) break;
+        top = fmaxf(fmaxf(S.red[it & 1][0][row], S.red[it & 1][1][row]),
+                    fmaxf(S.red[it & 1][2][row], S.red[it & 1][3][row]));
+        // the maximum moves on a rise of more than 2^kLazy only (weights up to
+        // 2^8 lose nothing in 32 bits), so O is rescaled on few tiles
+        float alpha = 1.f;
+        if (top > m + kLazy || m == -INFINITY) {
+          alpha = m == -INFINITY ? 1.f : ex2_approx(m - top);
+          m = top;
+          l *= alpha;
+        }
+        const float sub = m == -INFINITY ? 0.f : m;
+        uint32_t w[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          // weights are rounded to bf16 for the matrix product, the sum takes them as they are
+          const float a = ex2_approx(x[2 * j] - sub), b = ex2_approx(x[2 * j + 1] - sub);
+          l += a + b;
+          w[j] = pack_bf16(a, b);
+        }
+        if (it > 0) ok = mbar_wait_cluster(&S.pv_done, (it - 1) & 1);  // P is read, O settled
+        tc_fence_after();
+        if (tile == g.tile0) {
+          float z[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) z[j] = 0.f;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_st32(lanes + half * 128 + c * 32, z);
+          tmem_wait_st();
+        } else if (__any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            float o[32];
+            tmem_ld32(lanes + half * 128 + c * 32, o);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] *= alpha;
+            tmem_st32(lanes + half * 128 + c * 32, o);
+          }
+          tmem_wait_st();
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          *reinterpret_cast<uint4*>(S.p[page] + row * 128 + (((half * 4 + c) ^ (row & 7)) << 4)) =
+              make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+        fence_proxy_async_smem();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_at(p_bar);
+      }
+      if (!ok) break;
+      // the four threads of a row add up their sums; O is complete
+      S.red[it & 1][page * 2 + half][row] = l;
+      ok = mbar_wait_cluster(&S.pv_done, (it - 1) & 1);
+      if (!(ok = named_bar_all(1, kSoftmaxThreads, ok))) break;
+      tc_fence_after();
+      l = S.red[it & 1][0][row] + S.red[it & 1][1][row] + S.red[it & 1][2][row] + S.red[it & 1][3][row];
+      named_bar_sync(1, kSoftmaxThreads);  // red is written again by the next tile
+      const int64_t head = live ? (group - token * p.group_per_token) * 16 + (row & 15) : 0;
+      const int dv = half * 256 + page * 128;  // the 128 columns of O in these lanes
+      float* part = p.parts + (g.block + pair) * kSlotFloats;
+      const bool whole = g.whole;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        float o[32];
+        tmem_ld32(lanes + half * 128 + c * 32, o);
+        if (!live) continue;
+        if (whole) {
+          uint4* dst = reinterpret_cast<uint4*>(p.out + token * p.out_st + head * p.out_sh + dv + c * 32);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            dst[j] = make_uint4(pack_bf16(o[8 * j] * inv, o[8 * j + 1] * inv), pack_bf16(o[8 * j + 2] * inv, o[8 * j + 3] * inv),
+                                pack_bf16(o[8 * j + 4] * inv, o[8 * j + 5] * inv), pack_bf16(o[8 * j + 6] * inv, o[8 * j + 7] * inv));
+        } else {
+          float4* dst = reinterpret_cast<float4*>(part + (rank * kRows + row) * 512 + dv + c * 32);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) __stcg(dst + j, make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]));
+        }
+      }
+      if (live && half == 0 && page == 0) {
+        if (whole) {
+          p.lse[token * p.lse_st + head * p.lse_sh] = l == 0.f ? -INFINITY : m + log2f(l);
+        } else {
+          __stcg(part + 2 * kRows * 512 + rank * kRows + row, m);
+          __stcg(part + 2 * kRows * 512 + 2 * kRows + rank * kRows + row, l);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&S.seg_empty[n & 1]);
+    }
+    if (!ok) set_error(p.err, kErrTimeout);
   }
-  if (tid < 16) p.lse[t * p.lse_st + (h0 + tid) * p.lse_sh] = S.l[tid] == 0.f ? -INFINITY : S.m[tid] + log2f(S.l[tid]);
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // neither CTA leaves while the pair's MMAs or arrivals may reach it
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, 512);
+  }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+// ----------------------------------------------------------------- merge
+// Rows whose block several pairs share: with partials (O_k, m_k, l_k),
+//   o = sum_k 2^(m_k - M) O_k / sum_k 2^(m_k - M) l_k.
+// A CTA of 8 warps takes 8 / kStreams rows of the row block that boundary
+// blockIdx.y + 1 cuts (the first boundary inside it), kStreams warps a row.
+template <int kStreams>
+__global__ void __launch_bounds__(256) dsa_prefix_merge_kernel(const PrefixParams p) {
+  __shared__ float4 acc[kStreams > 1 ? 8 : 1][128];
+  __shared__ float ml[8][2];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long tiles = p.cum[p.blocks];
+  const int pairs = pairs_used(p, tiles), cut = blockIdx.y + 1;
+  if (cut >= pairs) return;
+  const long long at = pair_start(tiles, pairs, cut);
+  int64_t lo = 0, hi = p.blocks;
+  while (hi - lo > 1) {
+    const int64_t mid = (lo + hi) >> 1;
+    if (p.cum[mid] <= at)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  const long long c0 = p.cum[lo], c1 = p.cum[lo + 1];
+  if (at == c0 || pair_start(tiles, pairs, cut - 1) > c0) return;  // no cut inside, or not its first
+  const int first = pair_of(tiles, pairs, c0), last = pair_of(tiles, pairs, c1 - 1);
+  const int row = blockIdx.x * (8 / kStreams) + warp / kStreams, stream = warp % kStreams;
+  const int64_t group = lo * kGroups + (row >> 4);
+  if (group - (row >> 4) + (blockIdx.x * (8 / kStreams) >> 4) >= p.groups) return;  // rows of a CTA are in one group
+  const float* parts = p.parts + lo * kSlotFloats;
+  float m = -INFINITY, l = 0.f;
+  float4 o[4] = {};
+  for (int k = first + stream; k <= last; k += kStreams) {
+    const float* part = parts + (int64_t)k * kSlotFloats;
+    const float mk = __ldcg(part + 2 * kRows * 512 + row), lk = __ldcg(part + 2 * kRows * 512 + 2 * kRows + row);
+    float4 v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = __ldcg(reinterpret_cast<const float4*>(part + (int64_t)row * 512) + j * 32 + lane);
+    const float top = fmaxf(m, mk);
+    const float a = m == -INFINITY ? 0.f : exp2f(m - top), b = mk == -INFINITY ? 0.f : exp2f(mk - top);
+    m = top;
+    l = l * a + lk * b;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      o[j].x = o[j].x * a + v[j].x * b;
+      o[j].y = o[j].y * a + v[j].y * b;
+      o[j].z = o[j].z * a + v[j].z * b;
+      o[j].w = o[j].w * a + v[j].w * b;
+    }
+  }
+  if (kStreams > 1) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[warp][j * 32 + lane] = o[j];
+    if (lane == 0) {
+      ml[warp][0] = m;
+      ml[warp][1] = l;
+    }
+    __syncthreads();
+    if (stream != 0) return;
+    for (int s = 1; s < kStreams; ++s) {
+      const float mk = ml[warp + s][0], lk = ml[warp + s][1];
+      const float top = fmaxf(m, mk);
+      const float a = m == -INFINITY ? 0.f : exp2f(m - top), b = mk == -INFINITY ? 0.f : exp2f(mk - top);
+      m = top;
+      l = l * a + lk * b;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float4 v = acc[warp + s][j * 32 + lane];
+        o[j].x = o[j].x * a + v.x * b;
+        o[j].y = o[j].y * a + v.y * b;
+        o[j].z = o[j].z * a + v.z * b;
+        o[j].w = o[j].w * a + v.w * b;
+      }
+    }
+  }
+  const int64_t token = group / p.group_per_token, head = (group - token * p.group_per_token) * 16 + (row & 15);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    *reinterpret_cast<uint2*>(p.out + token * p.out_st + head * p.out_sh + (j * 32 + lane) * 4) =
+        make_uint2(pack_bf16(o[j].x * inv, o[j].y * inv), pack_bf16(o[j].z * inv, o[j].w * inv));
+  if (lane == 0) p.lse[token * p.lse_st + head * p.lse_sh] = l == 0.f ? -INFINITY : m + log2f(l);
+}
+
+// ------------------------------------------------------------------ host
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+  static std::once_flag once;
+  static EncodeTiledFn fn = nullptr;
+  std::call_once(once, [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(f);
+  });
+  return fn;
+}
+
+// bf16 [d2][d1][width] with element strides; a box is 64 values of `rows` of d1.
+bool encode(CUtensorMap* map, const void* base, int64_t width, int64_t d1, int64_t d2, int64_t s1, int64_t s2, int rows) {
+  EncodeTiledFn enc = encode_fn();
+  if (!enc) return false;
+  const cuuint64_t dims[3] = {(cuuint64_t)width, (cuuint64_t)d1, (cuuint64_t)d2};
+  const cuuint64_t strides[2] = {(cuuint64_t)s1 * 2, (cuuint64_t)s2 * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)rows, 1}, step[3] = {1, 1, 1};
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, step,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Pairs of CTAs that fit on the current device at once (cached), 0 on an error.
+int resident_pairs() {
+  static std::mutex mu;
+  static int cached[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  std::lock_guard<std::mutex> lock(mu);
+  if (cached[dev] == 0) {
+    int sms = 0;
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+    if (cudaFuncSetAttribute(dsa_prefix_attention_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)sizeof(PairSmem)) != cudaSuccess)
+      return 0;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(sms / 2 * 2));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = sizeof(PairSmem);
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, dsa_prefix_attention_kernel, &cfg) != cudaSuccess || n < 1) return 0;
+    cached[dev] = n < sms / 2 ? n : sms / 2;
+  }
+  return cached[dev];
+}
+
+struct Layout {
+  int64_t blocks, cum, parts;
+  size_t bytes;
+};
+Layout workspace_layout(int64_t tokens, int64_t heads, int pairs) {
+  Layout w;
+  w.blocks = (tokens * (heads / 16) + kGroups - 1) / kGroups;
+  w.cum = 256;
+  w.parts = w.cum + ((w.blocks + 1) * 8 + 255) / 256 * 256;
+  // a row block that one pair finishes needs no partial, but has a number
+  w.bytes = (size_t)(w.parts + (w.blocks + pairs) * (int64_t)kSlotFloats * 4);
+  return w;
+}
+
+// Launch with programmatic dependence on the grid before it.
+template <typename... Params, typename... Args>
+cudaError_t launch_after(void (*kernel)(Params...), dim3 grid, unsigned threads, size_t smem, cudaStream_t stream,
+                         Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 }  // namespace
@@ -135,7 +776,11 @@ extern "C" int dsa_shared_prefix_attention_workspace_size(int64_t num_tokens, in
   if (!bytes) return report_error(DSA_ERR_INVALID_ARG, "NULL pointer argument");
   if (num_tokens < 0) return report_error(DSA_ERR_INVALID_ARG, "negative size");
   if (num_heads <= 0 || num_heads % 16) return report_error(DSA_ERR_INVALID_ARG, "heads must be a positive multiple of 16");
-  *bytes = 256;
+  if (num_tokens * (num_heads / 16) > INT32_MAX)
+    return report_error(DSA_ERR_UNSUPPORTED, "too many tokens");
+  const int pairs = resident_pairs();
+  if (pairs < 1) return report_error(DSA_ERR_CUDA, "cannot query how many CTA pairs fit on the device");
+  *bytes = workspace_layout(num_tokens, num_heads, pairs).bytes;
   return DSA_OK;
 }
 
@@ -148,39 +793,54 @@ extern "C" int dsa_shared_prefix_attention(
     const int32_t* token_lens, int64_t num_tokens, int64_t num_heads, int64_t num_pages, float sm_scale,
     void* output, int64_t out_stride_token, int64_t out_stride_head, float* lse, int64_t lse_stride_token,
     int64_t lse_stride_head, void* workspace, size_t workspace_bytes, void* stream) {
-  size_t need = 0;
-  const int rc = dsa_shared_prefix_attention_workspace_size(num_tokens, num_heads, &need);
-  if (rc != DSA_OK) return rc;
-  if (max_prefix_len < 0 || batch < 0 || max_pages < 0 || num_pages < 0)
+  if (num_tokens < 0 || max_prefix_len < 0 || batch < 0 || max_pages < 0 || num_pages < 0)
     return report_error(DSA_ERR_INVALID_ARG, "negative size");
+  if (num_heads <= 0 || num_heads % 16)
+    return report_error(DSA_ERR_INVALID_ARG, "heads must be a positive multiple of 16");
   if (num_tokens == 0) return DSA_OK;
+  if (num_tokens * (num_heads / 16) > INT32_MAX || max_prefix_len > INT32_MAX || num_pages > INT32_MAX)
+    return report_error(DSA_ERR_UNSUPPORTED, "tokens, rows and pages are counted in 32 bits");
   if (!q_nope || !q_pe || !ckv_cache || !kpe_cache || !token_lens || !output || !lse || !workspace ||
       (max_prefix_len > 0 && !prefix_pages) || (batch > 0 && max_pages > 0 && !block_table))
     return report_error(DSA_ERR_INVALID_ARG, "NULL pointer argument");
+  if (num_pages == 0) return report_error(DSA_ERR_UNSUPPORTED, "the cache has no pages");
   if (!token_request && batch < num_tokens)
     return report_error(DSA_ERR_INVALID_ARG, "without token_request the block table needs a row for every token");
-  for (const void* q : {q_nope, q_pe, ckv_cache, kpe_cache})
-    if (reinterpret_cast<uintptr_t>(q) & 15) return report_error(DSA_ERR_INVALID_ARG, "queries and caches must be 16-byte aligned");
-  for (int64_t s : {q_nope_stride_token, q_nope_stride_head, q_pe_stride_token, q_pe_stride_head, ckv_stride_page,
-                    ckv_stride_row, kpe_stride_page, kpe_stride_row})
-    if (s < 0 || s % 8) return report_error(DSA_ERR_INVALID_ARG, "query and cache strides must be multiples of 8 elements");
-  if ((reinterpret_cast<uintptr_t>(output) & 15) || out_stride_token % 8 || out_stride_head % 8)
-    return report_error(DSA_ERR_INVALID_ARG, "output rows must be 16-byte aligned");
-  if (workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255))
+  for (const void* q : {q_nope, q_pe, ckv_cache, kpe_cache, (const void*)output})
+    if (reinterpret_cast<uintptr_t>(q) & 15)
+      return report_error(DSA_ERR_INVALID_ARG, "queries, caches and output must be 16-byte aligned");
+  if (out_stride_token % 8 || out_stride_head % 8)
+    return report_error(DSA_ERR_INVALID_ARG, "output strides must be multiples of 8 elements");
+  // a stride over a single token or page is never used: any value will do
+  if (num_tokens == 1) {
+    q_nope_stride_token = num_heads * q_nope_stride_head;
+    q_pe_stride_token = num_heads * q_pe_stride_head;
+  }
+  if (num_pages == 1) {
+    ckv_stride_page = 64 * ckv_stride_row;
+    kpe_stride_page = 64 * kpe_stride_row;
+  }
+  const int64_t inner[4] = {q_nope_stride_head, q_pe_stride_head, ckv_stride_row, kpe_stride_row};
+  const int64_t outer[4] = {q_nope_stride_token, q_pe_stride_token, ckv_stride_page, kpe_stride_page};
+  for (int i = 0; i < 4; ++i) {
+    const int64_t width = i & 1 ? 64 : 512;
+    if (inner[i] < width || inner[i] % 8 || outer[i] < inner[i] || outer[i] % inner[i] || outer[i] >= (1LL << 39))
+      return report_error(DSA_ERR_INVALID_ARG,
+                          "heads and cache rows must be 16-byte aligned rows that do not overlap, with the stride of "
+                          "tokens and pages a multiple of theirs");
+  }
+  const int pairs = resident_pairs();
+  if (pairs < 1) return report_error(DSA_ERR_CUDA, "cannot query how many CTA pairs fit on the device");
+  const Layout w = workspace_layout(num_tokens, num_heads, pairs);
+  if (workspace_bytes < w.bytes || (reinterpret_cast<uintptr_t>(workspace) & 255))
     return report_error(DSA_ERR_WORKSPACE, "workspace too small or not 256-byte aligned");
+  CUtensorMap map_qn, map_qp, map_ckv, map_kpe;
+  if (!encode(&map_qn, q_nope, 512, num_heads, num_tokens, q_nope_stride_head, q_nope_stride_token, 16) ||
+      !encode(&map_qp, q_pe, 64, num_heads, num_tokens, q_pe_stride_head, q_pe_stride_token, 16) ||
+      !encode(&map_ckv, ckv_cache, 512, 64, num_pages, ckv_stride_row, ckv_stride_page, 64) ||
+      !encode(&map_kpe, kpe_cache, 64, 64, num_pages, kpe_stride_row, kpe_stride_page, 64))
+    return report_error(DSA_ERR_CUDA, "cannot encode a tensor map");
   PrefixParams p;
-  p.qn = static_cast<const __nv_bfloat16*>(q_nope);
-  p.qp = static_cast<const __nv_bfloat16*>(q_pe);
-  p.ckv = static_cast<const __nv_bfloat16*>(ckv_cache);
-  p.kpe = static_cast<const __nv_bfloat16*>(kpe_cache);
-  p.qn_st = q_nope_stride_token;
-  p.qn_sh = q_nope_stride_head;
-  p.qp_st = q_pe_stride_token;
-  p.qp_sh = q_pe_stride_head;
-  p.ckv_sp = ckv_stride_page;
-  p.ckv_sr = ckv_stride_row;
-  p.kpe_sp = kpe_stride_page;
-  p.kpe_sr = kpe_stride_row;
   p.prefix_pages = prefix_pages;
   p.prefix_len = prefix_len;
   p.block_table = block_table;
@@ -192,7 +852,10 @@ extern "C" int dsa_shared_prefix_attention(
   p.max_pages = max_pages;
   p.tokens = num_tokens;
   p.num_pages = num_pages;
-  p.heads = (int)num_heads;
+  p.group_per_token = (int)(num_heads / 16);
+  p.groups = num_tokens * p.group_per_token;
+  p.blocks = w.blocks;
+  p.max_pairs = pairs;
   p.scale_log2 = sm_scale * 1.44269504088896340736f;
   p.out = static_cast<__nv_bfloat16*>(output);
   p.out_st = out_stride_token;
@@ -201,12 +864,22 @@ extern "C" int dsa_shared_prefix_attention(
   p.lse_st = lse_stride_token;
   p.lse_sh = lse_stride_head;
   p.err = static_cast<int*>(workspace);
-  cudaError_t e = cudaFuncSetAttribute(dsa_prefix_attention_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       (int)sizeof(PreSmem));
-  if (e != cudaSuccess) return report_error(DSA_ERR_CUDA, cudaGetErrorString(e));
-  dsa_prefix_attention_kernel<<<dim3((unsigned)num_tokens, (unsigned)(num_heads / 16)), kPreThreads, sizeof(PreSmem),
-                                static_cast<cudaStream_t>(stream)>>>(p);
-  e = cudaGetLastError();
+  p.cum = reinterpret_cast<long long*>(static_cast<char*>(workspace) + w.cum);
+  p.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + w.parts);
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  dsa_prefix_plan_kernel<<<1, kPlanThreads, 0, s>>>(p);
+  cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess)
+    e = launch_after(dsa_prefix_attention_kernel, dim3(2 * pairs), kThreads, sizeof(PairSmem), s, map_qn, map_qp,
+                     map_ckv, map_kpe, p);
+  if (e == cudaSuccess && pairs > 1) {
+    // few row blocks: many pairs share each, and their partials are read by 8 warps a row
+    const int rows = (int)(p.groups < kGroups ? p.groups : kGroups) * 16;
+    if (w.blocks * 4 <= pairs)
+      e = launch_after(dsa_prefix_merge_kernel<8>, dim3(rows, pairs - 1), 256, 0, s, p);
+    else
+      e = launch_after(dsa_prefix_merge_kernel<1>, dim3(rows / 8, pairs - 1), 256, 0, s, p);
+  }
   if (e != cudaSuccess) return report_error(DSA_ERR_CUDA, cudaGetErrorString(e));
   return DSA_OK;
 }

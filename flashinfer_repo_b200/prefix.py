@@ -13,7 +13,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .kernel import HEAD_DIM_CKV, HEAD_DIM_KPE, NUM_HEADS, PAGE_SIZE, _rowmajor
+from .kernel import HEAD_DIM_CKV, HEAD_DIM_KPE, NUM_HEADS, PAGE_SIZE
 
 _workspaces: dict[int, list] = {}  # per device: every buffer handed out, the newest last
 _size_cache: dict[tuple, int] = {}
@@ -104,11 +104,14 @@ def shared_prefix_attention(q_nope, q_pe, ckv_cache, kpe_cache, prefix_pages, pr
         assert lse.shape == (tokens, heads) and lse.dtype == torch.float32
     if tokens == 0:
         return output, lse
+    assert num_pages > 0, "the cache has no pages"
     prefix_pages, token_lens = _int32(prefix_pages), _int32(token_lens)
     if block_table.dtype != torch.int32 or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
         block_table = block_table.to(torch.int32).contiguous()
-    q_nope, q_pe = _rowmajor(q_nope, 8), _rowmajor(q_pe, 8)
-    ckv_cache, kpe_cache = _rowmajor(ckv_cache, 8), _rowmajor(kpe_cache, 8)
+    q_nope = q_nope if _tiled(q_nope) else q_nope.contiguous()
+    q_pe = q_pe if _tiled(q_pe) else q_pe.contiguous()
+    assert _tiled(ckv_cache) and _tiled(kpe_cache), \
+        "cache rows must be contiguous, 16-byte aligned and apart, the page stride a multiple of the row stride"
     if workspace is None:
         workspace = _workspace(device, prefix_workspace_size(tokens, heads, device))
     elif not (workspace.is_cuda and workspace.device == device and workspace.dtype == torch.uint8
@@ -123,6 +126,13 @@ def shared_prefix_attention(q_nope, q_pe, ckv_cache, kpe_cache, prefix_pages, pr
                  heads, num_pages, float(sm_scale), output.data_ptr(), output.stride(0), output.stride(1),
                  lse.data_ptr(), lse.stride(0), lse.stride(1), workspace.data_ptr(), workspace.numel())
     return output, lse
+
+
+def _tiled(t: torch.Tensor) -> bool:
+    """Whether the TMA can read rows of t [A, B, width] where they are."""
+    outer, inner, last = t.stride()
+    ok = last == 1 and t.data_ptr() % 16 == 0 and inner % 8 == 0 and inner >= t.shape[2]
+    return ok and (t.shape[0] == 1 or (outer >= inner and outer % inner == 0))
 
 
 def _int32(t: torch.Tensor) -> torch.Tensor:

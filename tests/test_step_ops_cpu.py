@@ -77,7 +77,7 @@ def _prefix(q=X, q_st=16 * 512, cache=X, row=512, pages=X, max_prefix=64, table=
                16 * 512, 512, out, 16, 1, ws, nws, None)
 
 
-@pytest.mark.parametrize("kw", [dict(q=None), dict(q=X + 8), dict(q_st=4), dict(cache=None), dict(cache=X + 2),
+@pytest.mark.parametrize("kw", [dict(q=None), dict(q=X + 8), dict(q_st=4, tokens=2), dict(cache=None), dict(cache=X + 2),
                                 dict(row=516), dict(pages=None), dict(max_prefix=-1), dict(table=None),
                                 dict(lens=None), dict(out=None), dict(ws=None), dict(batch=0, request=None),
                                 dict(tokens=-1), dict(heads=24), dict(heads=0), dict(num_pages=-1)])
