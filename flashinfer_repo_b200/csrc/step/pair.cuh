@@ -45,12 +45,16 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity
     if (clock64() - t0 > kWaitBudgetCycles) return false;
   }
 }
-// Arrivals on a barrier given by its shared::cluster address (own or the other CTA's).
+// Arrivals on a barrier given by its shared::cluster address (own or the other
+// CTA's).  The first orders this thread's shared-memory accesses at CTA scope:
+// enough for data that the pair's MMA reads on the writer's own SM, once
+// fence.proxy.async has put it there.  A release at cluster scope instead cost
+// about 1000 cycles an arrival.  The second orders nothing.
 __device__ __forceinline__ void mbar_arrive_at(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 __device__ __forceinline__ void mbar_arrive_expect_tx_at(uint32_t cluster_addr, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.release.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(cluster_addr),
+  asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(cluster_addr),
                "r"(bytes)
                : "memory");
 }

@@ -150,7 +150,7 @@ struct PairSmem {
   Segment seg[2];
   int valid[4][2];  // rows of the two pages of the last tiles
   uint64_t q_full, q_empty, k_full[3], k_empty[3], v_full[2], v_empty[2], s_full[2], p_full, pv_done;
-  uint64_t seg_full[2], seg_empty[2];
+  uint64_t seg_full[2], seg_empty[2], valid_full[4];
   uint32_t tmem;
 };
 static_assert(sizeof(PairSmem) <= 232448, "shared memory of a CTA");
@@ -186,6 +186,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       mbar_init(&S.seg_full[i], 1);
       mbar_init(&S.seg_empty[i], 8 + 2 + (rank == 0));
     }
+    for (int i = 0; i < 4; ++i) mbar_init(&S.valid_full[i], 1);
     mbar_init(&S.p_full, 2 * kSoftmaxThreads / 32);
     mbar_init(&S.pv_done, 1);
     fence_mbar_init();
@@ -277,129 +278,153 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
   } else if (warp == 8 || warp == 10) {
     // ------------------------------------------------- loads: Q and K, or V
-    if (elect_one()) {
-      const uint32_t q_bar = cluster_map(smem_u32(&S.q_full), 0);
-      const uint32_t k_bar = cluster_map(smem_u32(&S.k_full[0]), 0), v_bar = cluster_map(smem_u32(&S.v_full[0]), 0);
-      const bool keys = warp == 8;
-      bool ok = true;
-      int it = 0;
-      for (int n = 0; ok; ++n) {
-        const Segment& g = S.seg[n & 1];
-        if (!mbar_wait(&S.seg_full[n & 1], (n >> 1) & 1)) {
+    // Lane i looks up page i of the next 16 tiles, a round ahead, so that no
+    // tile waits for its page ids.
+    const uint32_t q_bar = cluster_map(smem_u32(&S.q_full), 0);
+    const uint32_t k_bar = cluster_map(smem_u32(&S.k_full[0]), 0), v_bar = cluster_map(smem_u32(&S.v_full[0]), 0);
+    const bool keys = warp == 8;
+    bool ok = true;
+    int it = 0;
+    for (int n = 0; ok; ++n) {
+      const Segment& g = S.seg[n & 1];
+      if (!mbar_wait(&S.seg_full[n & 1], (n >> 1) & 1)) {
+        ok = false;
+        break;
+      }
+      const int count = __shfl_sync(0xffffffffu, (int)(g.tile1 - g.tile0), 0);
+      if (count <= 0) break;
+      auto look_up = [&](int first, int* id, int* rows) {  // page `lane` from tile `first` on
+        const int64_t k = 2 * (g.tile0 + first) + lane;
+        *id = 0;
+        *rows = 0;
+        if (first + (lane >> 1) >= count || k >= g.pages) return;
+        const int t = page_token(g, k);
+        const int64_t at = t < 0 ? k : k - (t ? g.own_end[t - 1] : g.pre_pages);
+        *id = t < 0 ? p.prefix_pages[at] : p.block_table[g.request[t] * p.bt_stride + at];
+        *rows = (int)min((int64_t)64, (t < 0 ? g.pre_rows : g.own_len[t]) - at * 64);
+      };
+      int next_id, next_rows, id = 0, rows = 0;
+      look_up(0, &next_id, &next_rows);
+      if (keys) {
+        if (!mbar_wait(&S.q_empty, (n & 1) ^ 1)) {
           ok = false;
           break;
         }
-        if (g.tile0 >= g.tile1) break;
-        if (keys) {
-          if (!mbar_wait(&S.q_empty, (n & 1) ^ 1)) {
-            ok = false;
-            break;
-          }
-          const int64_t first = g.block * kGroups + rank * 4;
-          const int have = (int)max((int64_t)0, min((int64_t)4, p.groups - first));
-          mbar_arrive_expect_tx_at(q_bar, have * 9 * 2048);
-          for (int i = 0; i < have; ++i) {
-            const int64_t t = (first + i) / p.group_per_token;
-            const int h = (int)((first + i) - t * p.group_per_token) * 16;
-            for (int j = 0; j < 8; ++j)
-              tma_load_3d_pair(smem_u32(S.q[j]) + i * 2048, &map_qn, j * 64, h, (int)t, q_bar);
-            tma_load_3d_pair(smem_u32(S.q[8]) + i * 2048, &map_qp, 0, h, (int)t, q_bar);
-          }
+        const int64_t first = g.block * kGroups + rank * 4;
+        const int have = (int)max((int64_t)0, min((int64_t)4, p.groups - first));
+        if (lane == 0) mbar_arrive_expect_tx_at(q_bar, have * 9 * 2048);
+        __syncwarp();
+        for (int i = lane; i < have * 9; i += 32) {
+          const int64_t group = first + i / 9, t = group / p.group_per_token;
+          const int h = (int)(group - t * p.group_per_token) * 16, j = i % 9;
+          tma_load_3d_pair(smem_u32(S.q[j]) + (i / 9) * 2048, j < 8 ? &map_qn : &map_qp, j < 8 ? j * 64 : 0, h, (int)t, q_bar);
         }
-        for (long long tile = g.tile0; tile < g.tile1 && ok; ++tile, ++it) {
-          int page[2], row[2], valid[2];  // row: coordinate that puts the valid rows at the end
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int64_t k = 2 * tile + i;
-            int id = -1, rows = 0;
-            if (k < g.pages) {
-              const int t = page_token(g, k);
-              const int64_t at = t < 0 ? k : k - (t ? g.own_end[t - 1] : g.pre_pages);
-              id = t < 0 ? p.prefix_pages[at] : p.block_table[g.request[t] * p.bt_stride + at];
-              rows = (int)min((int64_t)64, (t < 0 ? g.pre_rows : g.own_len[t]) - at * 64);
-              if (id < 0 || id >= p.num_pages) {
-                if (keys) set_error(p.err, kErrBadIndex);
-                rows = 0;
-              }
-            }
-            valid[i] = rows;
-            page[i] = rows ? id : 0;
-            row[i] = rows ? rows - 64 : 64;  // 64: nothing of the page, all zeros
+        __syncwarp();
+      }
+      for (int i = 0; i < count && ok; ++i, ++it) {
+        if ((i & 15) == 0) {
+          id = next_id;
+          rows = next_rows;
+          if (rows > 0 && (id < 0 || id >= p.num_pages)) {
+            if (keys) set_error(p.err, kErrBadIndex);
+            rows = 0;
           }
-          const uint32_t parity = (it & 1) ^ 1;
-          if (keys) {
+          if (rows == 0) id = 0;
+          look_up(i + 16, &next_id, &next_rows);
+        }
+        int page[2], row[2], valid[2];  // row: the coordinate that puts the valid rows at the tile's end
 #pragma unroll
-            for (int c = 0; c < 3; ++c) {
-              if (!mbar_wait(&S.k_empty[c], parity)) {
-                ok = false;
-                break;
-              }
+        for (int b = 0; b < 2; ++b) {
+          page[b] = __shfl_sync(0xffffffffu, id, 2 * (i & 15) + b);
+          valid[b] = __shfl_sync(0xffffffffu, rows, 2 * (i & 15) + b);
+          row[b] = valid[b] ? valid[b] - 64 : 64;  // 64: nothing of the page, all zeros
+        }
+        const uint32_t parity = (it & 1) ^ 1;
+        if (keys) {
+          const int my_page = rank ? page[1] : page[0], my_row = rank ? row[1] : row[0];
+#pragma unroll
+          for (int c = 0; c < 3; ++c) {
+            if (!mbar_wait(&S.k_empty[c], parity)) {
+              ok = false;
+              break;
+            }
+            if (elect_one()) {
               if (c == 0) {
                 S.valid[it & 3][0] = valid[0];
                 S.valid[it & 3][1] = valid[1];
+                mbar_arrive(&S.valid_full[it & 3]);
               }
               mbar_arrive_expect_tx_at(k_bar + 8 * c, kKChunk);
 #pragma unroll
               for (int b = 0; b < 3; ++b) {
                 const int j = 3 * c + b;
-                if (j < 8)
-                  tma_load_3d_pair(smem_u32(S.k[c]) + b * kPanel, &map_ckv, j * 64, row[rank], page[rank], k_bar + 8 * c);
-                else
-                  tma_load_3d_pair(smem_u32(S.k[c]) + b * kPanel, &map_kpe, 0, row[rank], page[rank], k_bar + 8 * c);
+                tma_load_3d_pair(smem_u32(S.k[c]) + b * kPanel, j < 8 ? &map_ckv : &map_kpe, j < 8 ? j * 64 : 0, my_row,
+                                 my_page, k_bar + 8 * c);
               }
             }
-          } else {
+            __syncwarp();
+          }
+        } else {
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              if (!mbar_wait(&S.v_empty[c], parity)) {
-                ok = false;
-                break;
-              }
+          for (int c = 0; c < 2; ++c) {
+            if (!mbar_wait(&S.v_empty[c], parity)) {
+              ok = false;
+              break;
+            }
+            if (elect_one()) {
               mbar_arrive_expect_tx_at(v_bar + 8 * c, kVChunk);
 #pragma unroll
               for (int b = 0; b < 4; ++b)  // page b / 2, columns 64 (b % 2) of this CTA's 128
                 tma_load_3d_pair(smem_u32(S.v[c]) + b * kPanel, &map_ckv, c * 256 + rank * 128 + (b & 1) * 64, row[b >> 1],
                                  page[b >> 1], v_bar + 8 * c);
             }
+            __syncwarp();
           }
         }
-        mbar_arrive(&S.seg_empty[n & 1]);
       }
-      if (!ok) set_error(p.err, kErrTimeout);
+      if (lane == 0) mbar_arrive(&S.seg_empty[n & 1]);
     }
-    __syncwarp();
+    if (!ok) set_error(p.err, kErrTimeout);
   } else if (warp == 9) {
     // ----------------------------------------------------------- MMA issue
-    if (rank == 0 && elect_one()) {
+    // The warp stays together and one elected lane issues: the operands are
+    // then the same for all lanes and need no detour through lane registers.
+    if (rank == 0) {
       constexpr uint32_t id_qk = umma_idesc(1, 1, 0, 0, 128, 128);
       constexpr uint32_t id_pv = umma_idesc(1, 1, 0, 1, 128, 256);
+      const uint32_t base = __shfl_sync(0xffffffffu, tmem, 0);
       const uint64_t q_desc = umma_desc(smem_u32(S.q[0]), 16, 1024, kSwizzle128B);
       const uint64_t k_desc = umma_desc(smem_u32(S.k[0]), 16, 1024, kSwizzle128B);
       const uint64_t p_desc = umma_desc(smem_u32(S.p[0]), 16, 1024, kSwizzle128B);
       const uint64_t v_desc = umma_desc(smem_u32(S.v[0]), kPanel, 1024, kSwizzle128B);
       bool ok = true;
-      int it = 0;               // tiles whose scores are issued
-      uint32_t off[2][4];       // lanes left alone by the two pages of the tile before
+      int it = 0;          // tiles whose scores are issued
+      uint32_t off[2][4];  // lanes left alone by the two pages of the tile before
       bool masked = false;
       auto weigh = [&](int i) -> bool {  // O += P V of tile i
         if (!mbar_wait_cluster(&S.p_full, i & 1)) return false;
-        tc_fence_after();
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           if (!mbar_wait_cluster(&S.v_full[c], i & 1)) return false;
           tc_fence_after();
+          if (elect_one()) {
+            if (masked) {
 #pragma unroll
-          for (int ks = 0; ks < 8; ++ks) {
-            const uint64_t a = p_desc + (((ks >> 2) * kPanel + (ks & 3) * 32) >> 4);
-            const uint64_t b = v_desc + ((c * kVChunk + (ks >> 2) * 2 * kPanel + (ks & 3) * 2048) >> 4);
-            if (masked)
-              umma_f16_pair_masked(tmem + c * 128, a, b, id_pv, off[ks >> 2]);
-            else
-              umma_f16_pair(tmem + c * 128, a, b, id_pv, 1u);
+              for (int ks = 0; ks < 8; ++ks)
+                umma_f16_pair_masked(base + c * 128, p_desc + (((ks >> 2) * kPanel + (ks & 3) * 32) >> 4),
+                                     v_desc + ((c * kVChunk + (ks >> 2) * 2 * kPanel + (ks & 3) * 2048) >> 4), id_pv,
+                                     off[ks >> 2]);
+            } else {
+#pragma unroll
+              for (int ks = 0; ks < 8; ++ks)
+                umma_f16_pair(base + c * 128, p_desc + (((ks >> 2) * kPanel + (ks & 3) * 32) >> 4),
+                              v_desc + ((c * kVChunk + (ks >> 2) * 2 * kPanel + (ks & 3) * 2048) >> 4), id_pv, 1u);
+            }
+            umma_commit_pair(&S.v_empty[c]);
+            if (c == 1) umma_commit_pair(&S.pv_done);
           }
-          umma_commit_pair(&S.v_empty[c]);
+          __syncwarp();
         }
-        umma_commit_pair(&S.pv_done);
         return true;
       };
       for (int n = 0; ok; ++n) {
@@ -413,12 +438,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           ok = false;
           break;
         }
-        if (g.tile0 >= g.tile1) break;
+        const int count = __shfl_sync(0xffffffffu, (int)(g.tile1 - g.tile0), 0);
+        if (count <= 0) break;
         if (!mbar_wait_cluster(&S.q_full, n & 1)) {
           ok = false;
           break;
         }
-        for (long long tile = g.tile0; tile < g.tile1 && ok; ++tile, ++it) {
+        for (int i = 0; i < count && ok; ++i, ++it) {
+          const uint32_t scores = base + kTmemS + 64 * (it & 1);
 #pragma unroll
           for (int c = 0; c < 3; ++c) {
             if (!mbar_wait_cluster(&S.k_full[c], it & 1)) {
@@ -426,38 +453,42 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
               break;
             }
             tc_fence_after();
+            if (elect_one()) {
 #pragma unroll
-            for (int j = 0; j < 12; ++j)
-              umma_f16_pair(tmem + kTmemS + 64 * (it & 1),
-                            q_desc + (((3 * c + (j >> 2)) * kPanel + (j & 3) * 32) >> 4),
-                            k_desc + ((c * kKChunk + (j >> 2) * kPanel + (j & 3) * 32) >> 4), id_qk,
-                            (c > 0 || j > 0) ? 1u : 0u);
-            umma_commit_pair(&S.k_empty[c]);
+              for (int j = 0; j < 12; ++j)
+                umma_f16_pair(scores, q_desc + (((3 * c + (j >> 2)) * kPanel + (j & 3) * 32) >> 4),
+                              k_desc + ((c * kKChunk + (j >> 2) * kPanel + (j & 3) * 32) >> 4), id_qk,
+                              (c > 0 || j > 0) ? 1u : 0u);
+              umma_commit_pair(&S.k_empty[c]);
+              if (c == 2) {
+                umma_commit_pair(&S.s_full[it & 1]);
+                if (i + 1 == count) umma_commit_pair(&S.q_empty);
+              }
+            }
+            __syncwarp();
           }
           if (!ok) break;
-          umma_commit_pair(&S.s_full[it & 1]);
-          if (tile + 1 == g.tile1) umma_commit_pair(&S.q_empty);
-          if (tile > g.tile0 && !weigh(it - 1)) {
+          if (i > 0 && !weigh(it - 1)) {
             ok = false;
             break;
           }
-          masked = false;
+          uint32_t any = 0;
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int64_t k = 2 * tile + i;
+          for (int b = 0; b < 2; ++b) {
+            const int64_t k = 2 * (g.tile0 + i) + b;
             const int t = k < g.pages ? page_token(g, k) : -1;
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-              off[i][w] = t < 0 ? 0u : g.mask[t][w];
-              masked |= off[i][w] != 0;
+              off[b][w] = __shfl_sync(0xffffffffu, t < 0 ? 0u : g.mask[t][w], 0);
+              any |= off[b][w];
             }
           }
+          masked = any != 0;
         }
-        mbar_arrive(&S.seg_empty[n & 1]);
+        if (lane == 0) mbar_arrive(&S.seg_empty[n & 1]);
       }
       if (!ok) set_error(p.err, kErrTimeout);
     }
-    __syncwarp();
   } else {
     // --------------------------------------------------- softmax, epilogue
     // Lane quarter q of TMEM: rows 32 (q & 1) + lane against page q >> 1; the
@@ -480,7 +511,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       float m = -INFINITY, l = 0.f;
       for (long long tile = g.tile0; tile < g.tile1; ++tile, ++it) {
         const int64_t k = 2 * tile + page;
-        ok = ok && mbar_wait_cluster(&S.s_full[it & 1], (it >> 1) & 1);
+        ok = ok && mbar_wait(&S.valid_full[it & 3], (it >> 2) & 1) && mbar_wait_cluster(&S.s_full[it & 1], (it >> 1) & 1);
         tc_fence_after();
         const int t = k < g.pages ? page_token(g, k) : -1;
         const bool sees = live && (t < 0 || t == mine);
@@ -515,6 +546,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           l += a + b;
           w[j] = pack_bf16(a, b);
         }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) asm volatile("" : "+r"(w[j]));  // done before the wait, not behind it
         if (it > 0) ok = mbar_wait_cluster(&S.pv_done, (it - 1) & 1);  // P is read, O settled
         tc_fence_after();
         if (tile == g.tile0) {
