@@ -42,7 +42,6 @@ constexpr int kThreads = 12 * 32;
 constexpr int kSoftmaxThreads = 256;
 constexpr uint32_t kTmemS = 256;               // TMEM columns: O 0-255, scores 256 and 320
 constexpr int kSlotFloats = 2 * kRows * 512 + 4 * kRows;  // partial: O, m, l of 128 rows
-constexpr int kPlanThreads = 1024;
 constexpr float kLazy = 8.f;  // the running maximum follows only a rise of more than 2^8
 
 struct PrefixParams {
@@ -55,7 +54,7 @@ struct PrefixParams {
   float* lse;
   int64_t lse_st, lse_sh;
   int* err;
-  long long* cum;  // [blocks + 1] tiles before each row block
+  long long* cum;  // [blocks + 1] tiles before each row block, for the merge grid
   float* parts;    // [blocks + max_pairs] partials
 };
 
@@ -89,56 +88,41 @@ __device__ __forceinline__ int pair_of(long long tiles, int pairs, long long u) 
   return (int)(((u + 1) * pairs - 1) / tiles);
 }
 
-// ------------------------------------------------------------------ plan
-// Tiles before every row block, from the lengths: one CTA, a scan.
-__global__ void __launch_bounds__(kPlanThreads) dsa_prefix_plan_kernel(const PrefixParams p) {
-  __shared__ long long sums[kPlanThreads / 32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t pre = (prefix_rows(p) + 63) >> 6;
-  long long base = 0;
-  for (int64_t b0 = 0; b0 < p.blocks; b0 += kPlanThreads) {
-    const int64_t b = b0 + threadIdx.x;
-    long long n = 0;
-    if (b < p.blocks) {
-      int64_t pages = pre;
-      const int64_t t0 = first_token(p, b);
-      const int nt = tokens_of(p, b);
-      for (int i = 0; i < nt; ++i) {
-        int64_t r;
-        bool bad = false;
-        pages += (own_rows(p, t0 + i, &r, &bad) + 63) >> 6;
-      }
-      n = max((pages + 1) >> 1, (int64_t)1);  // one at least: an empty row block still writes its rows
+// Tiles of a row block's page list: the prefix, then for every run of tokens of
+// the same request the pages that all of them see whole, once, and for every
+// token the pages that are left.
+__device__ long long tiles_of(const PrefixParams& p, int64_t block, int64_t pre_pages) {
+  const int64_t t0 = first_token(p, block);
+  const int nt = tokens_of(p, block);
+  int64_t pages = pre_pages;
+  for (int i = 0; i < nt;) {
+    int64_t request, r, least, sum = 0;
+    bool bad;
+    least = own_rows(p, t0 + i, &request, &bad);
+    sum = (least + 63) >> 6;
+    int n = 1;
+    for (; i + n < nt; ++n) {
+      const int64_t len = own_rows(p, t0 + i + n, &r, &bad);
+      if (r != request) break;
+      least = min(least, len);
+      sum += (len + 63) >> 6;
     }
-    long long x = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long a = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += a;
-    }
-    if (lane == 31) sums[warp] = x;
-    __syncthreads();
-    long long before = base, all = 0;
-    for (int w = 0; w < kPlanThreads / 32; ++w) {
-      if (w < warp) before += sums[w];
-      all += sums[w];
-    }
-    if (b < p.blocks) p.cum[b] = before + x - n;
-    base += all;
-    __syncthreads();
+    pages += sum - (n - 1) * (least >> 6);
+    i += n;
   }
-  if (threadIdx.x == 0) p.cum[p.blocks] = base;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  return max((pages + 1) >> 1, (int64_t)1);  // one at least: an empty row block still writes its rows
 }
 
 // ------------------------------------------------------------ attention
-// One pair's stretch of a row block's pages.
+// One pair's stretch of a row block's pages.  Span 2 i: the pages that the run of
+// tokens beginning with token i shares, span 2 i + 1: the other pages of token i.
 struct Segment {
-  int64_t block, request[kGroups];
-  long long tile0, tile1;  // within the row block
-  int64_t pre_pages, pre_rows, pages, own_end[kGroups], own_len[kGroups];
-  int tokens, whole;       // whole: no other pair works on the row block
-  uint32_t mask[kGroups][4];  // TMEM lanes that do not belong to token i, 64 rows of each CTA
+  int64_t block;
+  int tile0, count, whole;  // whole: no other pair works on the row block
+  int pre_pages, pre_rows, pages;
+  int end[2 * kGroups], from[2 * kGroups];      // last page + 1 in the list, first page of the request
+  int request[2 * kGroups], rows[2 * kGroups];  // rows of the request that the span's tokens see
+  uint8_t sees[2 * kGroups];                    // its 16-head groups of the block
 };
 
 struct PairSmem {
@@ -151,16 +135,22 @@ struct PairSmem {
   int valid[4][2];  // rows of the two pages of the last tiles
   uint64_t q_full, q_empty, k_full[3], k_empty[3], v_full[2], v_empty[2], s_full[2], p_full, pv_done;
   uint64_t seg_full[2], seg_empty[2], valid_full[4];
+  long long start;  // tiles before this pair's first row block
+  int64_t block;
+  long long sums[kThreads / 32];
   uint32_t tmem;
 };
 static_assert(sizeof(PairSmem) <= 232448, "shared memory of a CTA");
 
-// Own token of page k of the segment's list, -1 for a prefix page.
-__device__ __forceinline__ int page_token(const Segment& g, int64_t k) {
-  if (k < g.pre_pages) return -1;
-  int i = 0;
-  while (i + 1 < g.tokens && k >= g.own_end[i]) ++i;
-  return i;
+// Span of page k >= pre_pages of the segment's list, searched from `span` on.
+__device__ __forceinline__ int span_of(const Segment& g, int k, int span) {
+  while (span < 2 * kGroups - 1 && k >= g.end[span]) ++span;
+  return span;
+}
+// TMEM lanes (rows 0-31 and 32-63 of each CTA) of the groups that do not see the page.
+__device__ __forceinline__ uint32_t lanes_off(uint32_t sees, int word) {
+  const uint32_t two = ~sees >> (2 * word);
+  return (two & 1 ? 0xffffu : 0u) | (two & 2 ? 0xffff0000u : 0u);
 }
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
@@ -197,28 +187,51 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   cluster_sync_all();  // both CTAs' barriers and TMEM are there
   tc_fence_after();
   const uint32_t tmem = S.tmem;
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // the plan is written
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // what ran before is done
 
-  const long long tiles = p.cum[p.blocks];
+  // Every CTA adds up the tiles of all row blocks (each thread a stretch of
+  // them) and finds where its pair begins: cheaper than a grid that plans.
+  const int64_t pre = prefix_rows(p), pre_pages = (pre + 63) >> 6;
+  const int64_t stretch = (p.blocks + kThreads - 1) / kThreads;
+  const int64_t b0 = min(threadIdx.x * stretch, p.blocks), b1 = min(b0 + stretch, p.blocks);
+  long long mine = 0;
+  for (int64_t b = b0; b < b1; ++b) mine += tiles_of(p, b, pre_pages);
+  long long before = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long a = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += a;
+  }
+  if (lane == 31) S.sums[warp] = before;
+  __syncthreads();
+  before -= mine;
+  long long tiles = 0;
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) before += S.sums[w];
+    tiles += S.sums[w];
+  }
   const int pairs = pairs_used(p, tiles);
-  const long long u0 = pair < pairs ? pair_start(tiles, pairs, pair) : 0;
-  const long long u1 = pair < pairs ? pair_start(tiles, pairs, pair + 1) : 0;
+  const long long u0 = pair < pairs ? pair_start(tiles, pairs, pair) : tiles;
+  const long long u1 = pair < pairs ? pair_start(tiles, pairs, pair + 1) : tiles;
+  if (blockIdx.x == 0 || (before <= u0 && u0 < before + mine)) {
+    long long c = before;
+    for (int64_t b = b0; b < b1; ++b) {
+      const long long n = tiles_of(p, b, pre_pages);
+      if (blockIdx.x == 0) p.cum[b] = c;
+      if (c <= u0 && u0 < c + n) {
+        S.block = b;
+        S.start = c;
+      }
+      c += n;
+    }
+    if (blockIdx.x == 0 && b1 == p.blocks) p.cum[p.blocks] = tiles;
+  }
+  __syncthreads();
 
   if (warp == 11) {
     // ------------------------------------------------------------- segments
-    int64_t block = 0;
-    if (u0 < u1) {
-      int64_t lo = 0, hi = p.blocks;
-      while (hi - lo > 1) {
-        const int64_t mid = (lo + hi) >> 1;
-        if (p.cum[mid] <= u0)
-          lo = mid;
-        else
-          hi = mid;
-      }
-      block = lo;
-    }
-    long long u = u0;
+    int64_t block = S.block;
+    long long u = u0, c0 = S.start;
     for (int n = 0;; ++n) {
       const int s = n & 1;
       if (!mbar_wait(&S.seg_empty[s], ((n >> 1) & 1) ^ 1)) {
@@ -228,52 +241,71 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       Segment& g = S.seg[s];
       if (u >= u1) {  // no more: an empty segment ends the other roles
         if (lane == 0) {
-          g.tile0 = g.tile1 = 0;
+          g.count = 0;
           mbar_arrive(&S.seg_full[s]);
         }
         break;
       }
-      const long long c0 = p.cum[block], c1 = p.cum[block + 1];
       const int nt = tokens_of(p, block);
-      const int64_t t0 = first_token(p, block), pre = prefix_rows(p);
-      int64_t len = 0, req = 0, pages = 0;
+      const int64_t t0 = first_token(p, block);
+      int64_t len = 0, request = -1;
       bool bad = false;
-      if (lane < nt) {
-        len = own_rows(p, t0 + lane, &req, &bad);
-        pages = (len + 63) >> 6;
-      }
+      if (lane < nt) len = own_rows(p, t0 + lane, &request, &bad);
       if (bad) set_error(p.err, kErrBadIndex);
+      uint32_t sees = 0;  // groups of the block that are this token's
+      for (int i = 0; i < kGroups; ++i)
+        if (lane < nt && (block * kGroups + i) / p.group_per_token == t0 + lane) sees |= 1u << i;
+      // groups behind the last one are nobody's: their lanes may be written
+      const uint32_t nobody = p.groups - block * kGroups < kGroups ? 0xffu << (p.groups - block * kGroups) & 0xffu : 0u;
+      const int64_t left = __shfl_up_sync(0xffffffffu, request, 1);
+      const bool first = lane < nt && (lane == 0 || left != request);
+      const uint32_t firsts = __ballot_sync(0xffffffffu, first);
+      const int run = __popc(firsts & (0xffffffffu >> (31 - lane)));
+      int64_t least = len;
+      uint32_t run_sees = 0;
+      for (int i = 0; i < kGroups; ++i) {
+        const int r = __shfl_sync(0xffffffffu, run, i);
+        const int64_t l = __shfl_sync(0xffffffffu, len, i);
+        const uint32_t m = __shfl_sync(0xffffffffu, sees, i);
+        if (i < nt && r == run) {
+          least = min(least, l);
+          run_sees |= m;
+        }
+      }
+      const int shared = (int)(least >> 6), own = (int)((len + 63) >> 6) - shared, both = (first ? shared : 0) + own;
+      int end = lane < nt ? both : 0;
 #pragma unroll
       for (int o = 1; o < kGroups; o <<= 1) {
-        const int64_t a = __shfl_up_sync(0xffffffffu, pages, o);
-        if (lane >= o) pages += a;
+        const int a = __shfl_up_sync(0xffffffffu, end, o);
+        if (lane >= o) end += a;
       }
-      const int64_t pre_pages = (pre + 63) >> 6;
-      if (lane < nt) {
-        g.own_end[lane] = pre_pages + pages;
-        g.own_len[lane] = len;
-        g.request[lane] = req;
-        if (lane == nt - 1) g.pages = pre_pages + pages;
-        uint32_t off[4] = {0, 0, 0, 0};
-        for (int i = 0; i < kGroups; ++i) {
-          const int64_t group = block * kGroups + i;
-          // groups behind the last one are nobody's: their lanes may be written
-          if (group < p.groups && group / p.group_per_token != t0 + lane) off[i >> 1] |= 0xffffu << (16 * (i & 1));
-        }
-        for (int i = 0; i < 4; ++i) g.mask[lane][i] = off[i];
+      end += (int)pre_pages;
+      if (lane < kGroups) {
+        const int own_pages = lane < nt ? own : 0;
+        g.end[2 * lane] = end - own_pages;
+        g.end[2 * lane + 1] = end;
+        g.from[2 * lane] = 0;
+        g.from[2 * lane + 1] = shared;
+        g.request[2 * lane] = g.request[2 * lane + 1] = (int)request;
+        g.rows[2 * lane] = shared * 64;
+        g.rows[2 * lane + 1] = (int)min(len, (int64_t)INT32_MAX);
+        g.sees[2 * lane] = (uint8_t)(run_sees | nobody);
+        g.sees[2 * lane + 1] = (uint8_t)(sees | nobody);
       }
+      const int pages = __shfl_sync(0xffffffffu, end, kGroups - 1);
+      const long long c1 = c0 + max((pages + 1) >> 1, 1);
       if (lane == 0) {
         g.block = block;
-        g.tile0 = u - c0;
-        g.tile1 = min(u1, c1) - c0;
-        g.pre_pages = pre_pages;
-        g.pre_rows = pre;
-        g.tokens = nt;
+        g.tile0 = (int)(u - c0);
+        g.count = (int)(min(u1, c1) - u);
+        g.pre_pages = (int)pre_pages;
+        g.pre_rows = (int)pre;
+        g.pages = pages;
         g.whole = u == c0 && c1 <= u1;
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&S.seg_full[s]);
-      u = min(u1, c1);
+      u = c0 = min(u1, c1);
       ++block;
     }
   } else if (warp == 8 || warp == 10) {
@@ -291,17 +323,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         ok = false;
         break;
       }
-      const int count = __shfl_sync(0xffffffffu, (int)(g.tile1 - g.tile0), 0);
+      const int count = __shfl_sync(0xffffffffu, g.count, 0);
       if (count <= 0) break;
       auto look_up = [&](int first, int* id, int* rows) {  // page `lane` from tile `first` on
-        const int64_t k = 2 * (g.tile0 + first) + lane;
+        const int k = 2 * (g.tile0 + first) + lane;
         *id = 0;
         *rows = 0;
         if (first + (lane >> 1) >= count || k >= g.pages) return;
-        const int t = page_token(g, k);
-        const int64_t at = t < 0 ? k : k - (t ? g.own_end[t - 1] : g.pre_pages);
-        *id = t < 0 ? p.prefix_pages[at] : p.block_table[g.request[t] * p.bt_stride + at];
-        *rows = (int)min((int64_t)64, (t < 0 ? g.pre_rows : g.own_len[t]) - at * 64);
+        if (k < g.pre_pages) {
+          *id = p.prefix_pages[k];
+          *rows = min(64, g.pre_rows - k * 64);
+        } else {
+          const int i = span_of(g, k, 0), at = k - (i ? g.end[i - 1] : g.pre_pages) + g.from[i];
+          *id = p.block_table[g.request[i] * p.bt_stride + at];
+          *rows = min(64, g.rows[i] - at * 64);
+        }
       };
       int next_id, next_rows, id = 0, rows = 0;
       look_up(0, &next_id, &next_rows);
@@ -438,8 +474,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           ok = false;
           break;
         }
-        const int count = __shfl_sync(0xffffffffu, (int)(g.tile1 - g.tile0), 0);
+        const int count = __shfl_sync(0xffffffffu, g.count, 0);
         if (count <= 0) break;
+        int span = 0;
         if (!mbar_wait_cluster(&S.q_full, n & 1)) {
           ok = false;
           break;
@@ -475,11 +512,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           uint32_t any = 0;
 #pragma unroll
           for (int b = 0; b < 2; ++b) {
-            const int64_t k = 2 * (g.tile0 + i) + b;
-            const int t = k < g.pages ? page_token(g, k) : -1;
+            const int k = 2 * (g.tile0 + i) + b;
+            uint32_t sees = 0xff;
+            if (k >= g.pre_pages && k < g.pages) {
+              span = span_of(g, k, span);
+              sees = g.sees[span];
+            }
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-              off[b][w] = __shfl_sync(0xffffffffu, t < 0 ? 0u : g.mask[t][w], 0);
+              off[b][w] = __shfl_sync(0xffffffffu, lanes_off(sees, w), 0);
               any |= off[b][w];
             }
           }
@@ -503,18 +544,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const Segment& g = S.seg[n & 1];
       ok = mbar_wait(&S.seg_full[n & 1], (n >> 1) & 1);
       if (!named_bar_all(1, kSoftmaxThreads, ok)) break;
-      if (g.tile0 >= g.tile1) break;
+      const int count = g.count;
+      if (count <= 0) break;
       const int64_t group = g.block * kGroups + rank * 4 + (row >> 4);
       const bool live = group < p.groups;
       const int64_t token = live ? group / p.group_per_token : 0;
-      const int mine = live ? (int)(token - first_token(p, g.block)) : -2;  // its place in the block
+      const int my_bit = rank * 4 + (row >> 4);
       float m = -INFINITY, l = 0.f;
-      for (long long tile = g.tile0; tile < g.tile1; ++tile, ++it) {
-        const int64_t k = 2 * tile + page;
+      int span = 0;
+      for (int i = 0; i < count; ++i, ++it) {
+        const int k = 2 * (g.tile0 + i) + page;
         ok = ok && mbar_wait(&S.valid_full[it & 3], (it >> 2) & 1) && mbar_wait_cluster(&S.s_full[it & 1], (it >> 1) & 1);
         tc_fence_after();
-        const int t = k < g.pages ? page_token(g, k) : -1;
-        const bool sees = live && (t < 0 || t == mine);
+        bool sees = live;
+        if (k >= g.pre_pages && k < g.pages) {
+          span = span_of(g, k, span);
+          sees = live && ((g.sees[span] >> my_bit) & 1);
+        }
         // the page's rows are at the end of its 64 columns
         const int from = sees ? 64 - S.valid[it & 3][page] - 32 * half : 32;
         float x[32];
@@ -550,7 +596,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         for (int j = 0; j < 16; ++j) asm volatile("" : "+r"(w[j]));  // done before the wait, not behind it
         if (it > 0) ok = mbar_wait_cluster(&S.pv_done, (it - 1) & 1);  // P is read, O settled
         tc_fence_after();
-        if (tile == g.tile0) {
+        if (i == 0) {
           float z[32];
 #pragma unroll
           for (int j = 0; j < 32; ++j) z[j] = 0.f;
@@ -634,29 +680,36 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 // ----------------------------------------------------------------- merge
 // Rows whose block several pairs share: with partials (O_k, m_k, l_k),
 //   o = sum_k 2^(m_k - M) O_k / sum_k 2^(m_k - M) l_k.
-// A CTA of 8 warps takes 8 / kStreams rows of the row block that boundary
-// blockIdx.y + 1 cuts (the first boundary inside it), kStreams warps a row.
+// A CTA of 8 warps takes 8 / kStreams rows of a row block, kStreams warps a row.
+// The grid has a slice for every row block or, where those are more, for every
+// boundary between pairs: then the row block whose first cut the boundary is.
 template <int kStreams>
-__global__ void __launch_bounds__(256) dsa_prefix_merge_kernel(const PrefixParams p) {
+__global__ void __launch_bounds__(256) dsa_prefix_merge_kernel(const PrefixParams p, const int by_cut) {
   __shared__ float4 acc[kStreams > 1 ? 8 : 1][128];
   __shared__ float ml[8][2];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long tiles = p.cum[p.blocks];
-  const int pairs = pairs_used(p, tiles), cut = blockIdx.y + 1;
-  if (cut >= pairs) return;
-  const long long at = pair_start(tiles, pairs, cut);
-  int64_t lo = 0, hi = p.blocks;
-  while (hi - lo > 1) {
-    const int64_t mid = (lo + hi) >> 1;
-    if (p.cum[mid] <= at)
-      lo = mid;
-    else
-      hi = mid;
+  const int pairs = pairs_used(p, tiles);
+  int64_t lo = blockIdx.y;
+  if (by_cut) {
+    const int cut = blockIdx.y + 1;
+    if (cut >= pairs) return;
+    const long long at = pair_start(tiles, pairs, cut);
+    int64_t hi = p.blocks;
+    lo = 0;
+    while (hi - lo > 1) {
+      const int64_t mid = (lo + hi) >> 1;
+      if (p.cum[mid] <= at)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    if (at == p.cum[lo] || pair_start(tiles, pairs, cut - 1) > p.cum[lo]) return;  // no cut inside, or not the first
   }
   const long long c0 = p.cum[lo], c1 = p.cum[lo + 1];
-  if (at == c0 || pair_start(tiles, pairs, cut - 1) > c0) return;  // no cut inside, or not its first
   const int first = pair_of(tiles, pairs, c0), last = pair_of(tiles, pairs, c1 - 1);
+  if (first == last) return;  // one pair had it all and wrote the results
   const int row = blockIdx.x * (8 / kStreams) + warp / kStreams, stream = warp % kStreams;
   const int64_t group = lo * kGroups + (row >> 4);
   if (group - (row >> 4) + (blockIdx.x * (8 / kStreams) >> 4) >= p.groups) return;  // rows of a CTA are in one group
@@ -900,18 +953,16 @@ extern "C" int dsa_shared_prefix_attention(
   p.cum = reinterpret_cast<long long*>(static_cast<char*>(workspace) + w.cum);
   p.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + w.parts);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  dsa_prefix_plan_kernel<<<1, kPlanThreads, 0, s>>>(p);
-  cudaError_t e = cudaGetLastError();
-  if (e == cudaSuccess)
-    e = launch_after(dsa_prefix_attention_kernel, dim3(2 * pairs), kThreads, sizeof(PairSmem), s, map_qn, map_qp,
-                     map_ckv, map_kpe, p);
+  cudaError_t e = launch_after(dsa_prefix_attention_kernel, dim3(2 * pairs), kThreads, sizeof(PairSmem), s, map_qn, map_qp,
+                               map_ckv, map_kpe, p);
   if (e == cudaSuccess && pairs > 1) {
     // few row blocks: many pairs share each, and their partials are read by 8 warps a row
-    const int rows = (int)(p.groups < kGroups ? p.groups : kGroups) * 16;
+    const int rows = (int)(p.groups < kGroups ? p.groups : kGroups) * 16, by_cut = w.blocks >= pairs;
+    const unsigned slices = (unsigned)(by_cut ? pairs - 1 : w.blocks);
     if (w.blocks * 4 <= pairs)
-      e = launch_after(dsa_prefix_merge_kernel<8>, dim3(rows, pairs - 1), 256, 0, s, p);
+      e = launch_after(dsa_prefix_merge_kernel<8>, dim3(rows, slices), 256, 0, s, p, by_cut);
     else
-      e = launch_after(dsa_prefix_merge_kernel<1>, dim3(rows / 8, pairs - 1), 256, 0, s, p);
+      e = launch_after(dsa_prefix_merge_kernel<1>, dim3(rows / 8, slices), 256, 0, s, p, by_cut);
   }
   if (e != cudaSuccess) return report_error(DSA_ERR_CUDA, cudaGetErrorString(e));
   return DSA_OK;
