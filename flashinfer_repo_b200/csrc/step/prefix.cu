@@ -46,8 +46,10 @@ constexpr float kLazy = 8.f;  // the running maximum follows only a rise of more
 
 struct PrefixParams {
   const int32_t *prefix_pages, *prefix_len, *block_table, *token_request, *token_lens;
-  int64_t max_prefix, bt_stride, batch, max_pages, tokens, num_pages, groups, blocks;
-  int group_per_token, max_pairs;
+  int64_t bt_stride;
+  int max_prefix, batch, max_own, num_pages;  // max_own: rows that a row of the block table has room for
+  int groups, blocks, group_per_token, max_pairs;
+  int q_boxes;  // query loads of 64 rows
   float scale_log2;
   __nv_bfloat16* out;
   int64_t out_st, out_sh;
@@ -58,25 +60,24 @@ struct PrefixParams {
   float* parts;    // [blocks + max_pairs] partials
 };
 
-__device__ __forceinline__ int64_t prefix_rows(const PrefixParams& p) {
-  return p.prefix_len ? min(p.max_prefix, (int64_t)max(*p.prefix_len, 0)) : p.max_prefix;
+__device__ __forceinline__ int prefix_rows(const PrefixParams& p) {
+  return p.prefix_len ? min(p.max_prefix, max(*p.prefix_len, 0)) : p.max_prefix;
 }
-// Own rows of token t and its row of the block table; what does not fit the
+// Row of the block table of token t, and its own rows: what does not fit the
 // table is cut off.
-__device__ __forceinline__ int64_t own_rows(const PrefixParams& p, int64_t t, int64_t* request, bool* bad) {
-  const int64_t len = max(p.token_lens[t], 0), r = p.token_request ? p.token_request[t] : t;
-  *request = r;
-  if (len == 0) return 0;
-  const bool known = r >= 0 && r < p.batch;
-  *bad = !known || len > p.max_pages * 64;
-  return known ? min(len, p.max_pages * 64) : 0;
+__device__ __forceinline__ int request_of(const PrefixParams& p, int t) { return p.token_request ? p.token_request[t] : t; }
+__device__ __forceinline__ bool bad_rows(const PrefixParams& p, int request, int len) {
+  return len > 0 && (request < 0 || request >= p.batch || len > p.max_own);
 }
-__device__ __forceinline__ int64_t first_token(const PrefixParams& p, int64_t block) {
-  return block * kGroups / p.group_per_token;
+__device__ __forceinline__ int own_rows(const PrefixParams& p, int request, int len) {
+  return request >= 0 && request < p.batch ? min(max(len, 0), p.max_own) : 0;
 }
-__device__ __forceinline__ int tokens_of(const PrefixParams& p, int64_t block) {
-  const int64_t last = min((block + 1) * kGroups, p.groups) - 1;
-  return (int)(last / p.group_per_token - first_token(p, block)) + 1;
+__device__ __forceinline__ int first_token(const PrefixParams& p, int block) {
+  return (unsigned)block * kGroups / (unsigned)p.group_per_token;
+}
+__device__ __forceinline__ int tokens_of(const PrefixParams& p, int block) {
+  const unsigned last = min((unsigned)(block + 1) * kGroups, (unsigned)p.groups) - 1;
+  return (int)(last / (unsigned)p.group_per_token) - first_token(p, block) + 1;
 }
 // The pairs that work: one tile each at least.  Tile u of the U tiles belongs
 // to the pair c with start(c) <= u < start(c + 1).
@@ -91,34 +92,37 @@ __device__ __forceinline__ int pair_of(long long tiles, int pairs, long long u) 
 // Tiles of a row block's page list: the prefix, then for every run of tokens of
 // the same request the pages that all of them see whole, once, and for every
 // token the pages that are left.
-__device__ long long tiles_of(const PrefixParams& p, int64_t block, int64_t pre_pages) {
-  const int64_t t0 = first_token(p, block);
-  const int nt = tokens_of(p, block);
-  int64_t pages = pre_pages;
-  for (int i = 0; i < nt;) {
-    int64_t request, r, least, sum = 0;
-    bool bad;
-    least = own_rows(p, t0 + i, &request, &bad);
-    sum = (least + 63) >> 6;
-    int n = 1;
-    for (; i + n < nt; ++n) {
-      const int64_t len = own_rows(p, t0 + i + n, &r, &bad);
-      if (r != request) break;
-      least = min(least, len);
-      sum += (len + 63) >> 6;
-    }
-    pages += sum - (n - 1) * (least >> 6);
-    i += n;
+__device__ int tiles_of(const PrefixParams& p, int block, int pre_pages) {
+  const int t0 = first_token(p, block), nt = tokens_of(p, block);
+  int request[kGroups], len[kGroups];  // all loads first: they are in flight together
+#pragma unroll
+  for (int i = 0; i < kGroups; ++i) {
+    request[i] = i < nt ? request_of(p, t0 + i) : -1;
+    len[i] = i < nt ? p.token_lens[t0 + i] : 0;
   }
-  return max((pages + 1) >> 1, (int64_t)1);  // one at least: an empty row block still writes its rows
+  int pages = pre_pages, least = 0, more = 0;  // more: tokens of the run behind its first
+#pragma unroll
+  for (int i = 0; i < kGroups; ++i) {
+    const int own = own_rows(p, request[i], len[i]);
+    if (i > 0 && i < nt && request[i] == request[i - 1]) {
+      least = min(least, own);
+      ++more;
+    } else {
+      pages -= more * (least >> 6);
+      least = own;
+      more = 0;
+    }
+    pages += (int)(((unsigned)own + 63) >> 6);
+  }
+  pages -= more * (least >> 6);
+  return max((pages + 1) >> 1, 1);  // one at least: an empty row block still writes its rows
 }
 
 // ------------------------------------------------------------ attention
 // One pair's stretch of a row block's pages.  Span 2 i: the pages that the run of
 // tokens beginning with token i shares, span 2 i + 1: the other pages of token i.
 struct Segment {
-  int64_t block;
-  int tile0, count, whole;  // whole: no other pair works on the row block
+  int block, tile0, count, whole;  // whole: no other pair works on the row block
   int pre_pages, pre_rows, pages;
   int end[2 * kGroups], from[2 * kGroups];      // last page + 1 in the list, first page of the request
   int request[2 * kGroups], rows[2 * kGroups];  // rows of the request that the span's tokens see
@@ -136,8 +140,8 @@ struct PairSmem {
   uint64_t q_full, q_empty, k_full[3], k_empty[3], v_full[2], v_empty[2], s_full[2], p_full, pv_done;
   uint64_t seg_full[2], seg_empty[2], valid_full[4];
   long long start;  // tiles before this pair's first row block
-  int64_t block;
   long long sums[kThreads / 32];
+  int block;
   uint32_t tmem;
 };
 static_assert(sizeof(PairSmem) <= 232448, "shared memory of a CTA");
@@ -155,8 +159,8 @@ __device__ __forceinline__ uint32_t lanes_off(uint32_t sees, int word) {
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     dsa_prefix_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __grid_constant__ CUtensorMap map_qp,
-                                const __grid_constant__ CUtensorMap map_ckv, const __grid_constant__ CUtensorMap map_kpe,
-                                const __grid_constant__ PrefixParams p) {
+                                const __grid_constant__ CUtensorMap map_ckv3, const __grid_constant__ CUtensorMap map_ckv2,
+                                const __grid_constant__ CUtensorMap map_kpe, const __grid_constant__ PrefixParams p) {
   extern __shared__ __align__(1024) uint8_t raw[];
   PairSmem& S = *reinterpret_cast<PairSmem*>(raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -191,11 +195,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
   // Every CTA adds up the tiles of all row blocks (each thread a stretch of
   // them) and finds where its pair begins: cheaper than a grid that plans.
-  const int64_t pre = prefix_rows(p), pre_pages = (pre + 63) >> 6;
-  const int64_t stretch = (p.blocks + kThreads - 1) / kThreads;
-  const int64_t b0 = min(threadIdx.x * stretch, p.blocks), b1 = min(b0 + stretch, p.blocks);
+  const int pre = prefix_rows(p), pre_pages = (int)(((unsigned)pre + 63) >> 6);
+  const int stretch = (p.blocks + kThreads - 1) / kThreads;
+  const int b0 = min((int)threadIdx.x * stretch, p.blocks), b1 = min(b0 + stretch, p.blocks);
   long long mine = 0;
-  for (int64_t b = b0; b < b1; ++b) mine += tiles_of(p, b, pre_pages);
+  for (int b = b0; b < b1; ++b) mine += tiles_of(p, b, pre_pages);
   long long before = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -215,8 +219,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const long long u1 = pair < pairs ? pair_start(tiles, pairs, pair + 1) : tiles;
   if (blockIdx.x == 0 || (before <= u0 && u0 < before + mine)) {
     long long c = before;
-    for (int64_t b = b0; b < b1; ++b) {
-      const long long n = tiles_of(p, b, pre_pages);
+    for (int b = b0; b < b1; ++b) {
+      const long long n = stretch == 1 ? mine : tiles_of(p, b, pre_pages);
       if (blockIdx.x == 0) p.cum[b] = c;
       if (c <= u0 && u0 < c + n) {
         S.block = b;
@@ -230,7 +234,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
   if (warp == 11) {
     // ------------------------------------------------------------- segments
-    int64_t block = S.block;
+    int block = S.block;
     long long u = u0, c0 = S.start;
     for (int n = 0;; ++n) {
       const int s = n & 1;
@@ -246,49 +250,51 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
         break;
       }
-      const int nt = tokens_of(p, block);
-      const int64_t t0 = first_token(p, block);
-      int64_t len = 0, request = -1;
-      bool bad = false;
-      if (lane < nt) len = own_rows(p, t0 + lane, &request, &bad);
-      if (bad) set_error(p.err, kErrBadIndex);
-      uint32_t sees = 0;  // groups of the block that are this token's
-      for (int i = 0; i < kGroups; ++i)
-        if (lane < nt && (block * kGroups + i) / p.group_per_token == t0 + lane) sees |= 1u << i;
-      // groups behind the last one are nobody's: their lanes may be written
-      const uint32_t nobody = p.groups - block * kGroups < kGroups ? 0xffu << (p.groups - block * kGroups) & 0xffu : 0u;
-      const int64_t left = __shfl_up_sync(0xffffffffu, request, 1);
+      const int nt = tokens_of(p, block), t0 = first_token(p, block);
+      int len = 0, request = -1;
+      if (lane < nt) {
+        request = request_of(p, t0 + lane);
+        len = p.token_lens[t0 + lane];
+      }
+      if (bad_rows(p, request, len)) set_error(p.err, kErrBadIndex);
+      len = own_rows(p, request, len);
+      // groups of the block that are this token's; those behind the last one
+      // are nobody's and their lanes may be written
+      const int g0 = (t0 + lane) * p.group_per_token - block * kGroups;
+      const uint32_t sees = lane < nt ? (0xffu << max(g0, 0)) & (0xffu >> max(kGroups - g0 - p.group_per_token, 0)) : 0u;
+      const int behind = p.groups - block * kGroups;
+      const uint32_t nobody = behind < kGroups ? 0xffu << behind & 0xffu : 0u;
+      const int left = __shfl_up_sync(0xffffffffu, request, 1);
       const bool first = lane < nt && (lane == 0 || left != request);
       const uint32_t firsts = __ballot_sync(0xffffffffu, first);
       const int run = __popc(firsts & (0xffffffffu >> (31 - lane)));
-      int64_t least = len;
+      int least = len;
       uint32_t run_sees = 0;
       for (int i = 0; i < kGroups; ++i) {
-        const int r = __shfl_sync(0xffffffffu, run, i);
-        const int64_t l = __shfl_sync(0xffffffffu, len, i);
+        const int r = __shfl_sync(0xffffffffu, run, i), l = __shfl_sync(0xffffffffu, len, i);
         const uint32_t m = __shfl_sync(0xffffffffu, sees, i);
         if (i < nt && r == run) {
           least = min(least, l);
           run_sees |= m;
         }
       }
-      const int shared = (int)(least >> 6), own = (int)((len + 63) >> 6) - shared, both = (first ? shared : 0) + own;
+      const int shared = least >> 6, own = (int)(((unsigned)len + 63) >> 6) - shared, both = (first ? shared : 0) + own;
       int end = lane < nt ? both : 0;
 #pragma unroll
       for (int o = 1; o < kGroups; o <<= 1) {
         const int a = __shfl_up_sync(0xffffffffu, end, o);
         if (lane >= o) end += a;
       }
-      end += (int)pre_pages;
+      end += pre_pages;
       if (lane < kGroups) {
         const int own_pages = lane < nt ? own : 0;
         g.end[2 * lane] = end - own_pages;
         g.end[2 * lane + 1] = end;
         g.from[2 * lane] = 0;
         g.from[2 * lane + 1] = shared;
-        g.request[2 * lane] = g.request[2 * lane + 1] = (int)request;
+        g.request[2 * lane] = g.request[2 * lane + 1] = request;
         g.rows[2 * lane] = shared * 64;
-        g.rows[2 * lane + 1] = (int)min(len, (int64_t)INT32_MAX);
+        g.rows[2 * lane + 1] = len;
         g.sees[2 * lane] = (uint8_t)(run_sees | nobody);
         g.sees[2 * lane + 1] = (uint8_t)(sees | nobody);
       }
@@ -298,8 +304,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         g.block = block;
         g.tile0 = (int)(u - c0);
         g.count = (int)(min(u1, c1) - u);
-        g.pre_pages = (int)pre_pages;
-        g.pre_rows = (int)pre;
+        g.pre_pages = pre_pages;
+        g.pre_rows = pre;
         g.pages = pages;
         g.whole = u == c0 && c1 <= u1;
       }
@@ -346,14 +352,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           ok = false;
           break;
         }
-        const int64_t first = g.block * kGroups + rank * 4;
-        const int have = (int)max((int64_t)0, min((int64_t)4, p.groups - first));
-        if (lane == 0) mbar_arrive_expect_tx_at(q_bar, have * 9 * 2048);
-        __syncwarp();
-        for (int i = lane; i < have * 9; i += 32) {
-          const int64_t group = first + i / 9, t = group / p.group_per_token;
-          const int h = (int)(group - t * p.group_per_token) * 16, j = i % 9;
-          tma_load_3d_pair(smem_u32(S.q[j]) + (i / 9) * 2048, j < 8 ? &map_qn : &map_qp, j < 8 ? j * 64 : 0, h, (int)t, q_bar);
+        // boxes of whole tokens or of whole quarters of the 64 rows; what lies
+        // behind the last token is filled with zeros
+        if (elect_one()) {
+          mbar_arrive_expect_tx_at(q_bar, 9 * kPanel);
+          for (int i = 0; i < p.q_boxes; ++i) {
+            const unsigned group = g.block * kGroups + rank * 4 + i * (4 / p.q_boxes);
+            const int t = group / (unsigned)p.group_per_token, h = (group - t * p.group_per_token) * 16;
+            if (p.q_boxes == 1) {
+              tma_load_4d_pair(smem_u32(S.q[0]), &map_qn, 0, h, t, 0, q_bar);
+            } else {
+              for (int j = 0; j < 8; ++j)
+                tma_load_4d_pair(smem_u32(S.q[j]) + i * (kPanel / p.q_boxes), &map_qn, 0, h, t, j, q_bar);
+            }
+            tma_load_4d_pair(smem_u32(S.q[8]) + i * (kPanel / p.q_boxes), &map_qp, 0, h, t, 0, q_bar);
+          }
         }
         __syncwarp();
       }
@@ -391,12 +404,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 mbar_arrive(&S.valid_full[it & 3]);
               }
               mbar_arrive_expect_tx_at(k_bar + 8 * c, kKChunk);
-#pragma unroll
-              for (int b = 0; b < 3; ++b) {
-                const int j = 3 * c + b;
-                tma_load_3d_pair(smem_u32(S.k[c]) + b * kPanel, j < 8 ? &map_ckv : &map_kpe, j < 8 ? j * 64 : 0, my_row,
-                                 my_page, k_bar + 8 * c);
-              }
+              tma_load_4d_pair(smem_u32(S.k[c]), c < 2 ? &map_ckv3 : &map_ckv2, 0, my_row, 3 * c, my_page, k_bar + 8 * c);
+              if (c == 2) tma_load_4d_pair(smem_u32(S.k[2]) + 2 * kPanel, &map_kpe, 0, my_row, 0, my_page, k_bar + 16);
             }
             __syncwarp();
           }
@@ -410,9 +419,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             if (elect_one()) {
               mbar_arrive_expect_tx_at(v_bar + 8 * c, kVChunk);
 #pragma unroll
-              for (int b = 0; b < 4; ++b)  // page b / 2, columns 64 (b % 2) of this CTA's 128
-                tma_load_3d_pair(smem_u32(S.v[c]) + b * kPanel, &map_ckv, c * 256 + rank * 128 + (b & 1) * 64, row[b >> 1],
-                                 page[b >> 1], v_bar + 8 * c);
+              for (int b = 0; b < 2; ++b)  // this CTA's 128 of 256 columns, as two panels a page
+                tma_load_4d_pair(smem_u32(S.v[c]) + b * 2 * kPanel, &map_ckv2, 0, row[b], c * 4 + rank * 2, page[b],
+                                 v_bar + 8 * c);
             }
             __syncwarp();
           }
@@ -546,9 +555,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if (!named_bar_all(1, kSoftmaxThreads, ok)) break;
       const int count = g.count;
       if (count <= 0) break;
-      const int64_t group = g.block * kGroups + rank * 4 + (row >> 4);
+      const int group = g.block * kGroups + rank * 4 + (row >> 4);
       const bool live = group < p.groups;
-      const int64_t token = live ? group / p.group_per_token : 0;
+      const int token = live ? (unsigned)group / (unsigned)p.group_per_token : 0;
       const int my_bit = rank * 4 + (row >> 4);
       float m = -INFINITY, l = 0.f;
       int span = 0;
@@ -631,9 +640,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       tc_fence_after();
       l = S.red[it & 1][0][row] + S.red[it & 1][1][row] + S.red[it & 1][2][row] + S.red[it & 1][3][row];
       named_bar_sync(1, kSoftmaxThreads);  // red is written again by the next tile
-      const int64_t head = live ? (group - token * p.group_per_token) * 16 + (row & 15) : 0;
+      const int head = live ? (group - token * p.group_per_token) * 16 + (row & 15) : 0;
       const int dv = half * 256 + page * 128;  // the 128 columns of O in these lanes
-      float* part = p.parts + (g.block + pair) * kSlotFloats;
+      float* part = p.parts + (int64_t)(g.block + pair) * kSlotFloats;
       const bool whole = g.whole;
       const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
@@ -648,9 +657,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             dst[j] = make_uint4(pack_bf16(o[8 * j] * inv, o[8 * j + 1] * inv), pack_bf16(o[8 * j + 2] * inv, o[8 * j + 3] * inv),
                                 pack_bf16(o[8 * j + 4] * inv, o[8 * j + 5] * inv), pack_bf16(o[8 * j + 6] * inv, o[8 * j + 7] * inv));
         } else {
-          float4* dst = reinterpret_cast<float4*>(part + (rank * kRows + row) * 512 + dv + c * 32);
+          // partials lie as [512 / 4][128 rows][4]: the lanes of a warp store side by side
+          float4* dst = reinterpret_cast<float4*>(part) + (dv + c * 32) / 4 * (2 * kRows) + rank * kRows + row;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) __stcg(dst + j, make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]));
+          for (int j = 0; j < 8; ++j)
+            __stcg(dst + j * (2 * kRows), make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]));
         }
       }
       if (live && half == 0 && page == 0) {
@@ -680,26 +691,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 // ----------------------------------------------------------------- merge
 // Rows whose block several pairs share: with partials (O_k, m_k, l_k),
 //   o = sum_k 2^(m_k - M) O_k / sum_k 2^(m_k - M) l_k.
-// A CTA of 8 warps takes 8 / kStreams rows of a row block, kStreams warps a row.
+// A CTA takes 8 rows of a row block and 32 of its 128 column quads: thread i the
+// row i % 8, so that 8 rows of a quad are read as one line.
 // The grid has a slice for every row block or, where those are more, for every
 // boundary between pairs: then the row block whose first cut the boundary is.
-template <int kStreams>
-__global__ void __launch_bounds__(256) dsa_prefix_merge_kernel(const PrefixParams p, const int by_cut) {
-  __shared__ float4 acc[kStreams > 1 ? 8 : 1][128];
-  __shared__ float ml[8][2];
+constexpr int kMergeRows = 8, kMergeQuads = 32;  // rows and column quads of a CTA
+
+__global__ void __launch_bounds__(kMergeRows * kMergeQuads)
+    dsa_prefix_merge_kernel(const PrefixParams p, const int by_cut) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long tiles = p.cum[p.blocks];
   const int pairs = pairs_used(p, tiles);
-  int64_t lo = blockIdx.y;
+  int lo = blockIdx.y;
   if (by_cut) {
     const int cut = blockIdx.y + 1;
     if (cut >= pairs) return;
     const long long at = pair_start(tiles, pairs, cut);
-    int64_t hi = p.blocks;
+    int hi = p.blocks;
     lo = 0;
     while (hi - lo > 1) {
-      const int64_t mid = (lo + hi) >> 1;
+      const int mid = (lo + hi) >> 1;
       if (p.cum[mid] <= at)
         lo = mid;
       else
@@ -707,65 +718,53 @@ __global__ void __launch_bounds__(256) dsa_prefix_merge_kernel(const PrefixParam
     }
     if (at == p.cum[lo] || pair_start(tiles, pairs, cut - 1) > p.cum[lo]) return;  // no cut inside, or not the first
   }
-  const long long c0 = p.cum[lo], c1 = p.cum[lo + 1];
-  const int first = pair_of(tiles, pairs, c0), last = pair_of(tiles, pairs, c1 - 1);
+  const int first = pair_of(tiles, pairs, p.cum[lo]), last = pair_of(tiles, pairs, p.cum[lo + 1] - 1);
   if (first == last) return;  // one pair had it all and wrote the results
-  const int row = blockIdx.x * (8 / kStreams) + warp / kStreams, stream = warp % kStreams;
-  const int64_t group = lo * kGroups + (row >> 4);
-  if (group - (row >> 4) + (blockIdx.x * (8 / kStreams) >> 4) >= p.groups) return;  // rows of a CTA are in one group
-  const float* parts = p.parts + lo * kSlotFloats;
+  const int row = blockIdx.x / (128 / kMergeQuads) * kMergeRows + threadIdx.x % kMergeRows;
+  const int quad = blockIdx.x % (128 / kMergeQuads) * kMergeQuads + threadIdx.x / kMergeRows;
+  const int group = lo * kGroups + (row >> 4);
+  if (group >= p.groups) return;
   float m = -INFINITY, l = 0.f;
-  float4 o[4] = {};
-  for (int k = first + stream; k <= last; k += kStreams) {
-    const float* part = parts + (int64_t)k * kSlotFloats;
-    const float mk = __ldcg(part + 2 * kRows * 512 + row), lk = __ldcg(part + 2 * kRows * 512 + 2 * kRows + row);
-    float4 v[4];
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  constexpr int kAhead = 8;  // partials whose loads are in flight together
+  for (int k0 = first; k0 <= last; k0 += kAhead) {
+    float mk[kAhead], lk[kAhead];
+    float4 v[kAhead];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = __ldcg(reinterpret_cast<const float4*>(part + (int64_t)row * 512) + j * 32 + lane);
-    const float top = fmaxf(m, mk);
-    const float a = m == -INFINITY ? 0.f : exp2f(m - top), b = mk == -INFINITY ? 0.f : exp2f(mk - top);
-    m = top;
-    l = l * a + lk * b;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      o[j].x = o[j].x * a + v[j].x * b;
-      o[j].y = o[j].y * a + v[j].y * b;
-      o[j].z = o[j].z * a + v[j].z * b;
-      o[j].w = o[j].w * a + v[j].w * b;
-    }
-  }
-  if (kStreams > 1) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) acc[warp][j * 32 + lane] = o[j];
-    if (lane == 0) {
-      ml[warp][0] = m;
-      ml[warp][1] = l;
-    }
-    __syncthreads();
-    if (stream != 0) return;
-    for (int s = 1; s < kStreams; ++s) {
-      const float mk = ml[warp + s][0], lk = ml[warp + s][1];
-      const float top = fmaxf(m, mk);
-      const float a = m == -INFINITY ? 0.f : exp2f(m - top), b = mk == -INFINITY ? 0.f : exp2f(mk - top);
-      m = top;
-      l = l * a + lk * b;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float4 v = acc[warp + s][j * 32 + lane];
-        o[j].x = o[j].x * a + v.x * b;
-        o[j].y = o[j].y * a + v.y * b;
-        o[j].z = o[j].z * a + v.z * b;
-        o[j].w = o[j].w * a + v.w * b;
+    for (int i = 0; i < kAhead; ++i) {
+      mk[i] = -INFINITY;
+      lk[i] = 0.f;
+      v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (k0 + i <= last) {
+        const float* part = p.parts + (int64_t)(lo + k0 + i) * kSlotFloats;
+        mk[i] = __ldcg(part + 2 * kRows * 512 + row);
+        lk[i] = __ldcg(part + 2 * kRows * 512 + 2 * kRows + row);
+        v[i] = __ldcg(reinterpret_cast<const float4*>(part) + quad * (2 * kRows) + row);
       }
     }
-  }
-  const int64_t token = group / p.group_per_token, head = (group - token * p.group_per_token) * 16 + (row & 15);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+    float top = m;
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
-    *reinterpret_cast<uint2*>(p.out + token * p.out_st + head * p.out_sh + (j * 32 + lane) * 4) =
-        make_uint2(pack_bf16(o[j].x * inv, o[j].y * inv), pack_bf16(o[j].z * inv, o[j].w * inv));
-  if (lane == 0) p.lse[token * p.lse_st + head * p.lse_sh] = l == 0.f ? -INFINITY : m + log2f(l);
+    for (int i = 0; i < kAhead; ++i) top = fmaxf(top, mk[i]);
+    const float a = m == -INFINITY ? 0.f : exp2f(m - top);
+    m = top;
+    l *= a;
+    o = make_float4(o.x * a, o.y * a, o.z * a, o.w * a);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const float b = mk[i] == -INFINITY ? 0.f : exp2f(mk[i] - top);
+      l += lk[i] * b;
+      o.x += v[i].x * b;
+      o.y += v[i].y * b;
+      o.z += v[i].z * b;
+      o.w += v[i].w * b;
+    }
+  }
+  const int token = (unsigned)group / (unsigned)p.group_per_token;
+  const int head = (group - token * p.group_per_token) * 16 + (row & 15);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  *reinterpret_cast<uint2*>(p.out + token * p.out_st + head * p.out_sh + quad * 4) =
+      make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+  if (quad == 0) p.lse[token * p.lse_st + head * p.lse_sh] = l == 0.f ? -INFINITY : m + log2f(l);
 }
 
 // ------------------------------------------------------------------ host
@@ -786,14 +785,16 @@ EncodeTiledFn encode_fn() {
   return fn;
 }
 
-// bf16 [d2][d1][width] with element strides; a box is 64 values of `rows` of d1.
-bool encode(CUtensorMap* map, const void* base, int64_t width, int64_t d1, int64_t d2, int64_t s1, int64_t s2, int rows) {
+// bf16 rows of 64 values: dimensions 1 to 3 with their strides in elements, and
+// the box of them that one load takes.
+bool encode(CUtensorMap* map, const void* base, int64_t n1, int64_t s1, int b1, int64_t n2, int64_t s2, int b2, int64_t n3,
+            int64_t s3, int b3) {
   EncodeTiledFn enc = encode_fn();
   if (!enc) return false;
-  const cuuint64_t dims[3] = {(cuuint64_t)width, (cuuint64_t)d1, (cuuint64_t)d2};
-  const cuuint64_t strides[2] = {(cuuint64_t)s1 * 2, (cuuint64_t)s2 * 2};
-  const cuuint32_t box[3] = {64, (cuuint32_t)rows, 1}, step[3] = {1, 1, 1};
-  return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, step,
+  const cuuint64_t dims[4] = {64, (cuuint64_t)n1, (cuuint64_t)n2, (cuuint64_t)n3};
+  const cuuint64_t strides[3] = {(cuuint64_t)s1 * 2, (cuuint64_t)s2 * 2, (cuuint64_t)s3 * 2};
+  const cuuint32_t box[4] = {64, (cuuint32_t)b1, (cuuint32_t)b2, (cuuint32_t)b3}, step[4] = {1, 1, 1, 1};
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, step,
              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -862,7 +863,7 @@ extern "C" int dsa_shared_prefix_attention_workspace_size(int64_t num_tokens, in
   if (!bytes) return report_error(DSA_ERR_INVALID_ARG, "NULL pointer argument");
   if (num_tokens < 0) return report_error(DSA_ERR_INVALID_ARG, "negative size");
   if (num_heads <= 0 || num_heads % 16) return report_error(DSA_ERR_INVALID_ARG, "heads must be a positive multiple of 16");
-  if (num_tokens * (num_heads / 16) > INT32_MAX)
+  if (num_tokens * (num_heads / 16) > (1 << 30))
     return report_error(DSA_ERR_UNSUPPORTED, "too many tokens");
   const int pairs = resident_pairs();
   if (pairs < 1) return report_error(DSA_ERR_CUDA, "cannot query how many CTA pairs fit on the device");
@@ -884,7 +885,7 @@ extern "C" int dsa_shared_prefix_attention(
   if (num_heads <= 0 || num_heads % 16)
     return report_error(DSA_ERR_INVALID_ARG, "heads must be a positive multiple of 16");
   if (num_tokens == 0) return DSA_OK;
-  if (num_tokens * (num_heads / 16) > INT32_MAX || max_prefix_len > INT32_MAX || num_pages > INT32_MAX)
+  if (num_tokens * (num_heads / 16) > (1 << 30) || max_prefix_len > INT32_MAX || num_pages > INT32_MAX)
     return report_error(DSA_ERR_UNSUPPORTED, "tokens, rows and pages are counted in 32 bits");
   if (!q_nope || !q_pe || !ckv_cache || !kpe_cache || !token_lens || !output || !lse || !workspace ||
       (max_prefix_len > 0 && !prefix_pages) || (batch > 0 && max_pages > 0 && !block_table))
@@ -920,11 +921,17 @@ extern "C" int dsa_shared_prefix_attention(
   const Layout w = workspace_layout(num_tokens, num_heads, pairs);
   if (workspace_bytes < w.bytes || (reinterpret_cast<uintptr_t>(workspace) & 255))
     return report_error(DSA_ERR_WORKSPACE, "workspace too small or not 256-byte aligned");
-  CUtensorMap map_qn, map_qp, map_ckv, map_kpe;
-  if (!encode(&map_qn, q_nope, 512, num_heads, num_tokens, q_nope_stride_head, q_nope_stride_token, 16) ||
-      !encode(&map_qp, q_pe, 64, num_heads, num_tokens, q_pe_stride_head, q_pe_stride_token, 16) ||
-      !encode(&map_ckv, ckv_cache, 512, 64, num_pages, ckv_stride_row, ckv_stride_page, 64) ||
-      !encode(&map_kpe, kpe_cache, 64, 64, num_pages, kpe_stride_row, kpe_stride_page, 64))
+  // a query box holds whole tokens (of at most 64 heads), 64 heads of one, or 32 or 16
+  const int gpt = (int)(num_heads / 16);
+  const int box_groups = gpt % 4 == 0 ? 4 : gpt % 2 == 0 ? 2 : 1, box_tokens = box_groups == gpt ? 4 / gpt : 1;
+  const int q_boxes = 4 / (box_groups * box_tokens);
+  CUtensorMap map_qn, map_qp, map_ckv3, map_ckv2, map_kpe;
+  if (!encode(&map_qn, q_nope, num_heads, q_nope_stride_head, 16 * box_groups, num_tokens, q_nope_stride_token, box_tokens, 8,
+              64, q_boxes == 1 ? 8 : 1) ||
+      !encode(&map_qp, q_pe, num_heads, q_pe_stride_head, 16 * box_groups, num_tokens, q_pe_stride_token, box_tokens, 1, 64, 1) ||
+      !encode(&map_ckv3, ckv_cache, 64, ckv_stride_row, 64, 8, 64, 3, num_pages, ckv_stride_page, 1) ||
+      !encode(&map_ckv2, ckv_cache, 64, ckv_stride_row, 64, 8, 64, 2, num_pages, ckv_stride_page, 1) ||
+      !encode(&map_kpe, kpe_cache, 64, kpe_stride_row, 64, 1, 64, 1, num_pages, kpe_stride_page, 1))
     return report_error(DSA_ERR_CUDA, "cannot encode a tensor map");
   PrefixParams p;
   p.prefix_pages = prefix_pages;
@@ -932,16 +939,16 @@ extern "C" int dsa_shared_prefix_attention(
   p.block_table = block_table;
   p.token_request = token_request;
   p.token_lens = token_lens;
-  p.max_prefix = max_prefix_len;
+  p.max_prefix = (int)max_prefix_len;
   p.bt_stride = block_table_stride;
-  p.batch = batch;
-  p.max_pages = max_pages;
-  p.tokens = num_tokens;
-  p.num_pages = num_pages;
-  p.group_per_token = (int)(num_heads / 16);
-  p.groups = num_tokens * p.group_per_token;
-  p.blocks = w.blocks;
+  p.batch = (int)(batch < INT32_MAX ? batch : INT32_MAX);
+  p.max_own = (int)(max_pages < INT32_MAX / 64 ? max_pages * 64 : INT32_MAX);
+  p.num_pages = (int)num_pages;
+  p.group_per_token = gpt;
+  p.groups = (int)(num_tokens * gpt);
+  p.blocks = (int)w.blocks;
   p.max_pairs = pairs;
+  p.q_boxes = q_boxes;
   p.scale_log2 = sm_scale * 1.44269504088896340736f;
   p.out = static_cast<__nv_bfloat16*>(output);
   p.out_st = out_stride_token;
@@ -954,15 +961,12 @@ extern "C" int dsa_shared_prefix_attention(
   p.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + w.parts);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e = launch_after(dsa_prefix_attention_kernel, dim3(2 * pairs), kThreads, sizeof(PairSmem), s, map_qn, map_qp,
-                               map_ckv, map_kpe, p);
+                               map_ckv3, map_ckv2, map_kpe, p);
   if (e == cudaSuccess && pairs > 1) {
-    // few row blocks: many pairs share each, and their partials are read by 8 warps a row
-    const int rows = (int)(p.groups < kGroups ? p.groups : kGroups) * 16, by_cut = w.blocks >= pairs;
-    const unsigned slices = (unsigned)(by_cut ? pairs - 1 : w.blocks);
-    if (w.blocks * 4 <= pairs)
-      e = launch_after(dsa_prefix_merge_kernel<8>, dim3(rows, slices), 256, 0, s, p, by_cut);
-    else
-      e = launch_after(dsa_prefix_merge_kernel<1>, dim3(rows / 8, slices), 256, 0, s, p, by_cut);
+    const int rows = (p.groups < kGroups ? p.groups : kGroups) * 16, by_cut = p.blocks >= pairs;
+    e = launch_after(dsa_prefix_merge_kernel,
+                     dim3(rows / kMergeRows * (128 / kMergeQuads), (unsigned)(by_cut ? pairs - 1 : p.blocks)),
+                     kMergeRows * kMergeQuads, 0, s, p, by_cut);
   }
   if (e != cudaSuccess) return report_error(DSA_ERR_CUDA, cudaGetErrorString(e));
   return DSA_OK;
