@@ -8,6 +8,8 @@ from __future__ import annotations
 import ctypes
 import os
 
+import torch
+
 from . import build as _build
 
 _lib = None
@@ -107,19 +109,35 @@ def call(fn_name: str, *args):
     check(fn_name, getattr(load(), fn_name)(*args))
 
 
-def call_on(device, fn_name: str, *args):
-    """`call` with `device` current and torch's current stream of that device
-    as the last argument."""
-    import torch
-    if device.index is None or device.index == torch.cuda.current_device():
-        check(fn_name, getattr(load(), fn_name)(*args, torch.cuda.current_stream(device).cuda_stream))
+_bound = {}
+
+
+def call_on(index: int, fn_name: str, *args):
+    """`call` with CUDA device `index` current and torch's current stream of that
+    device as the last argument."""
+    f = _bound.get(fn_name)
+    if f is None:
+        f = _bound[fn_name] = getattr(load(), fn_name)
+    # the raw getters: torch.cuda.current_stream builds an object, 1.5 us a call
+    if torch._C._cuda_getDevice() == index:
+        rc = f(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(device):
-            check(fn_name, getattr(load(), fn_name)(*args, torch.cuda.current_stream(device).cuda_stream))
+        with torch.cuda.device(index):
+            rc = f(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc != 0:
+        check(fn_name, rc)
 
 
-def check_cuda(device, **tensors):
-    """RuntimeError unless every tensor (None is skipped) is on the CUDA `device`."""
+def same_device(**tensors) -> int:
+    """Index of the one CUDA device that every tensor (None is skipped) is on;
+    RuntimeError if they are on several or on the CPU."""
+    index = -1
     for name, t in tensors.items():
-        if t is not None and (not t.is_cuda or t.device != device):
-            raise RuntimeError(f"{name} must be a CUDA tensor on {device} (no CPU path), got {t.device}")
+        if t is None:
+            continue
+        at = t.get_device()
+        if at != index or at < 0:
+            if index >= 0 or at < 0:
+                raise RuntimeError(f"{name} must be a CUDA tensor on the other tensors' device (no CPU path), got {t.device}")
+            index = at
+    return index

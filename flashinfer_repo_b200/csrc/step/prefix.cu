@@ -911,10 +911,9 @@ extern "C" int dsa_shared_prefix_attention(
   const int64_t outer[4] = {q_nope_stride_token, q_pe_stride_token, ckv_stride_page, kpe_stride_page};
   for (int i = 0; i < 4; ++i) {
     const int64_t width = i & 1 ? 64 : 512;
-    if (inner[i] < width || inner[i] % 8 || outer[i] < inner[i] || outer[i] % inner[i] || outer[i] >= (1LL << 39))
+    if (inner[i] < width || inner[i] % 8 || outer[i] < inner[i] || outer[i] % 8 || outer[i] >= (1LL << 39))
       return report_error(DSA_ERR_INVALID_ARG,
-                          "heads and cache rows must be 16-byte aligned rows that do not overlap, with the stride of "
-                          "tokens and pages a multiple of theirs");
+                          "heads and cache rows must be 16-byte aligned and must not overlap");
   }
   const int pairs = resident_pairs();
   if (pairs < 1) return report_error(DSA_ERR_CUDA, "cannot query how many CTA pairs fit on the device");

@@ -26,20 +26,20 @@ def latent_cache_append(kv, norm_weight, positions, slots, inv_freq, ckv_cache, 
     to bf16.  Slots must be distinct (-1 apart).  device_error: optional int32
     tensor that collects DSA_DEVERR_* bits (1: a slot outside the cache, skipped).
     """
-    assert kv.dim() == 2 and kv.shape[1] == HEAD_DIM_CKV + HEAD_DIM_KPE, "kv must be [tokens, 576]"
-    assert kv.dtype in DTYPES and norm_weight.dtype in DTYPES, "kv and norm_weight: bf16, fp16 or fp32"
-    assert norm_weight.shape == (HEAD_DIM_CKV,)
-    device, tokens = kv.device, kv.shape[0]
+    tokens, width = kv.shape
     num_pages = ckv_cache.shape[0]
-    assert ckv_cache.dtype == torch.bfloat16 and kpe_cache.dtype == torch.bfloat16
+    kv_type, norm_type = DTYPES.get(kv.dtype), DTYPES.get(norm_weight.dtype)
+    assert width == HEAD_DIM_CKV + HEAD_DIM_KPE, "kv must be [tokens, 576]"
+    assert kv_type is not None and norm_type is not None, "kv and norm_weight: bf16, fp16 or fp32"
+    assert norm_weight.shape == (HEAD_DIM_CKV,)
+    assert ckv_cache.dtype == torch.bfloat16 and kpe_cache.dtype == torch.bfloat16, "the caches are bf16"
     assert ckv_cache.shape == (num_pages, PAGE_SIZE, HEAD_DIM_CKV)
     assert kpe_cache.shape == (num_pages, PAGE_SIZE, HEAD_DIM_KPE)
-    assert ckv_cache.stride(2) == 1 and kpe_cache.stride(2) == 1, "cache rows must be contiguous"
-    assert slots.shape == (tokens,) and slots.dtype in (torch.int32, torch.int64)
+    assert slots.shape == (tokens,) and slots.dtype in (torch.int32, torch.int64), "slots must be [tokens] int32 or int64"
     assert inv_freq.shape == (HEAD_DIM_KPE // 2,), "inv_freq must have 32 values"
-    _lib.check_cuda(device, kv=kv, norm_weight=norm_weight, slots=slots, ckv_cache=ckv_cache,
-                    kpe_cache=kpe_cache, device_error=device_error)
-    positions, inv_freq = _check_rotation(device, positions, inv_freq, tokens, layout)
+    index = _lib.same_device(kv=kv, norm_weight=norm_weight, positions=positions, slots=slots, inv_freq=inv_freq,
+                             ckv_cache=ckv_cache, kpe_cache=kpe_cache, device_error=device_error)
+    positions, inv_freq = _check_rotation(positions, inv_freq, tokens, layout)
     if device_error is not None:
         assert device_error.dtype == torch.int32 and device_error.numel() >= 1, "device_error must be int32"
     if kv.stride(1) != 1:
@@ -47,9 +47,10 @@ def latent_cache_append(kv, norm_weight, positions, slots, inv_freq, ckv_cache, 
     norm_weight = norm_weight.contiguous()
     if slots.dtype != torch.int32 or not slots.is_contiguous():
         slots = slots.to(torch.int32).contiguous()
-    _lib.call_on(device, "dsa_latent_cache_append", kv.data_ptr(), kv.stride(0), DTYPES[kv.dtype],
-                 norm_weight.data_ptr(), DTYPES[norm_weight.dtype], tokens, positions.data_ptr(),
-                 int(positions.dtype == torch.int64), slots.data_ptr(), inv_freq.data_ptr(),
-                 ckv_cache.data_ptr(), ckv_cache.stride(0), ckv_cache.stride(1), kpe_cache.data_ptr(),
-                 kpe_cache.stride(0), kpe_cache.stride(1), num_pages, float(eps), LAYOUTS[layout],
-                 float(rope_scale), device_error.data_ptr() if device_error is not None else None)
+    c_page, c_row, c_last = ckv_cache.stride()
+    e_page, e_row, e_last = kpe_cache.stride()
+    assert c_last == 1 and e_last == 1, "cache rows must be contiguous"
+    _lib.call_on(index, "dsa_latent_cache_append", kv.data_ptr(), kv.stride(0), kv_type, norm_weight.data_ptr(), norm_type,
+                 tokens, positions.data_ptr(), positions.dtype == torch.int64, slots.data_ptr(), inv_freq.data_ptr(),
+                 ckv_cache.data_ptr(), c_page, c_row, kpe_cache.data_ptr(), e_page, e_row, num_pages, eps,
+                 LAYOUTS[layout], rope_scale, device_error.data_ptr() if device_error is not None else None)

@@ -48,31 +48,31 @@ def step_layout(seq_lens, query_lens, block_table, free_pages, num_tokens, *, pr
     of pages, table columns or rows; 1: a negative entry of an older page).
     Calling it again with the same lengths and free pages gives the same result.
     """
-    device = block_table.device
     seq_lens, query_lens = _lens(seq_lens, "seq_lens"), _lens(query_lens, "query_lens")
-    num_tokens = int(num_tokens)
-    batch = seq_lens.shape[0]
-    assert query_lens.shape[0] == batch and num_tokens >= 0
-    assert block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[0] == batch
-    assert block_table.shape[1] <= 1 or block_table.stride(1) == 1, "block_table rows must be contiguous"
     free_pages = _lens(free_pages, "free_pages")
-    _lib.check_cuda(device, block_table=block_table, seq_lens=seq_lens, query_lens=query_lens,
-                    free_pages=free_pages, prefix_len=prefix_len, device_error=device_error)
+    num_tokens = int(num_tokens)
+    batch, width = block_table.shape
+    assert seq_lens.shape[0] == batch and query_lens.shape[0] == batch and num_tokens >= 0
+    assert block_table.dtype == torch.int32 and (width <= 1 or block_table.stride(1) == 1), \
+        "block_table must be int32 with contiguous rows"
+    index = _lib.same_device(block_table=block_table, seq_lens=seq_lens, query_lens=query_lens, free_pages=free_pages,
+                             prefix_len=prefix_len, device_error=device_error)
     if prefix_len is not None:
         assert prefix_len.dtype == torch.int32 and prefix_len.numel() == 1, "prefix_len must be one int32"
     if device_error is not None:
         assert device_error.dtype == torch.int32 and device_error.numel() >= 1, "device_error must be int32"
     if out is None:
-        buf = torch.empty(4 * num_tokens + 1, dtype=torch.int32, device=device)
-        out = StepLayout(*buf.split((num_tokens,) * 4 + (1,)))
+        buf = block_table.new_empty(4 * num_tokens + 1)
+        out = StepLayout(*buf.split_with_sizes((num_tokens, num_tokens, num_tokens, num_tokens, 1)))
+        at = buf.data_ptr()
+        outs = tuple(at + 4 * num_tokens * i for i in range(5))
     else:
-        _lib.check_cuda(device, **out._asdict())
+        assert _lib.same_device(**out._asdict()) == index, "out: on the inputs' device"
         for t, n in zip(out, (num_tokens,) * 4 + (1,)):
             assert t.dtype == torch.int32 and t.numel() == n and t.is_contiguous(), "out: int32, contiguous"
-    _lib.call_on(device, "dsa_step_layout", seq_lens.data_ptr(), query_lens.data_ptr(), batch,
-                 block_table.data_ptr(), block_table.stride(0), block_table.shape[1], free_pages.data_ptr(),
+        outs = tuple(t.data_ptr() for t in out)
+    _lib.call_on(index, "dsa_step_layout", seq_lens.data_ptr(), query_lens.data_ptr(), batch,
+                 block_table.data_ptr(), block_table.stride(0), width, free_pages.data_ptr(),
                  free_pages.shape[0], prefix_len.data_ptr() if prefix_len is not None else None, num_tokens,
-                 out.slots.data_ptr(), out.positions.data_ptr(), out.token_request.data_ptr(),
-                 out.token_lens.data_ptr(), out.pages_used.data_ptr(),
-                 device_error.data_ptr() if device_error is not None else None)
+                 *outs, device_error.data_ptr() if device_error is not None else None)
     return out

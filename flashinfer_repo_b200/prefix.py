@@ -20,10 +20,9 @@ _size_cache: dict[tuple, int] = {}
 
 
 def prefix_workspace_size(num_tokens: int, heads: int = NUM_HEADS, device=None) -> int:
-    """Bytes of the workspace that a call of this shape needs on `device`
-    (default: the current device)."""
-    device = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
-    index = device.index if device.index is not None else torch.cuda.current_device()
+    """Bytes of the workspace that a call of this shape needs on `device` (an
+    index or torch.device; default: the current device)."""
+    index = _index(device)
     nbytes = _size_cache.get((index, num_tokens, heads))
     if nbytes is None:
         n = ctypes.c_size_t(0)
@@ -33,15 +32,25 @@ def prefix_workspace_size(num_tokens: int, heads: int = NUM_HEADS, device=None) 
     return nbytes
 
 
-def _workspace(device, nbytes):
-    """The device's shared workspace.  A larger call gets a new buffer; older
-    ones are kept, since a captured graph may hold their address."""
-    kept = _workspaces.setdefault(device.index, [])
+def _index(device) -> int:
+    if isinstance(device, int):
+        return device
+    index = torch.device(device).index if device is not None else None
+    return index if index is not None else torch.cuda.current_device()
+
+
+def _workspace(index: int, nbytes: int) -> torch.Tensor:
+    """The device's shared workspace.  A larger call gets a new buffer, half as
+    large again at least; older ones are kept, since a captured graph may hold
+    their address."""
+    kept = _workspaces.setdefault(index, [])
     if not kept or kept[-1].numel() < nbytes:
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("the workspace must grow during stream capture: make one call of this size before "
-                               "the capture, or pass workspace=")
-        kept.append(torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device))
+        nbytes = max(nbytes, kept[-1].numel() * 3 // 2 // 256 * 256 if kept else 0)
+        with torch.cuda.device(index):
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("the workspace must grow during stream capture: make one call of this size before "
+                                   "the capture, or pass workspace=")
+            kept.append(torch.zeros(nbytes, dtype=torch.uint8, device=f"cuda:{index}"))
     return kept[-1]
 
 
@@ -71,16 +80,17 @@ def shared_prefix_attention(q_nope, q_pe, ckv_cache, kpe_cache, prefix_pages, pr
     assert dim == HEAD_DIM_CKV and q_pe.shape == (tokens, heads, HEAD_DIM_KPE)
     assert ckv_cache.shape == (num_pages, PAGE_SIZE, HEAD_DIM_CKV)
     assert kpe_cache.shape == (num_pages, PAGE_SIZE, HEAD_DIM_KPE)
-    assert block_table.dim() == 2 and prefix_pages.dim() == 1 and token_lens.shape == (tokens,)
-    device = q_nope.device
     length = prefix_len if isinstance(prefix_len, torch.Tensor) else None
-    _lib.check_cuda(device, q_nope=q_nope, q_pe=q_pe, ckv_cache=ckv_cache, kpe_cache=kpe_cache,
-                    prefix_pages=prefix_pages, prefix_len=length, block_table=block_table, token_lens=token_lens,
-                    token_request=token_request, output=output, lse=lse)
-    for name, t in (("q_nope", q_nope), ("q_pe", q_pe), ("ckv_cache", ckv_cache), ("kpe_cache", kpe_cache)):
-        assert t.dtype == torch.bfloat16, f"{name} must be bfloat16"
-    for name, t in (("prefix_pages", prefix_pages), ("block_table", block_table), ("token_lens", token_lens)):
-        assert t.dtype in (torch.int32, torch.int64), f"{name} must be int32 or int64"
+    index = _lib.same_device(q_nope=q_nope, q_pe=q_pe, ckv_cache=ckv_cache, kpe_cache=kpe_cache,
+                             prefix_pages=prefix_pages, prefix_len=length, block_table=block_table,
+                             token_lens=token_lens, token_request=token_request, output=output, lse=lse,
+                             workspace=workspace)
+    bf16 = torch.bfloat16
+    assert q_nope.dtype == bf16 and q_pe.dtype == bf16 and ckv_cache.dtype == bf16 and kpe_cache.dtype == bf16, \
+        "queries and caches must be bfloat16"
+    requests, width = block_table.shape
+    assert token_lens.shape == (tokens,), "token_lens must be [tokens]"
+    prefix_pages, token_lens = _int32(prefix_pages, "prefix_pages"), _int32(token_lens, "token_lens")
     if length is not None:
         assert length.numel() == 1 and length.dtype == torch.int32, "prefix_len must be an int or one int32"
         bound = prefix_pages.shape[0] * PAGE_SIZE
@@ -88,62 +98,66 @@ def shared_prefix_attention(q_nope, q_pe, ckv_cache, kpe_cache, prefix_pages, pr
         bound = int(prefix_len)
         assert 0 <= bound <= prefix_pages.shape[0] * PAGE_SIZE, "prefix_len does not fit prefix_pages"
     if token_request is not None:
-        assert token_request.shape == (tokens,) and token_request.dtype in (torch.int32, torch.int64)
-        token_request = _int32(token_request)
+        assert token_request.shape == (tokens,), "token_request must be [tokens]"
+        token_request = _int32(token_request, "token_request")
     else:
-        assert block_table.shape[0] >= tokens, "without token_request the block table needs a row for every token"
+        assert requests >= tokens, "without token_request the block table needs a row for every token"
     if output is None:
-        output = torch.empty((tokens, heads, HEAD_DIM_CKV), dtype=torch.bfloat16, device=device)
+        output = q_nope.new_empty((tokens, heads, HEAD_DIM_CKV))
     else:
-        assert output.shape == (tokens, heads, HEAD_DIM_CKV) and output.dtype == torch.bfloat16
+        assert output.shape == (tokens, heads, HEAD_DIM_CKV) and output.dtype == bf16
         assert output.stride(-1) == 1 and output.stride(0) % 8 == 0 and output.stride(1) % 8 == 0 \
             and output.data_ptr() % 16 == 0, "output rows must be contiguous and 16-byte aligned"
     if lse is None:
-        lse = torch.empty((tokens, heads), dtype=torch.float32, device=device)
+        lse = q_nope.new_empty((tokens, heads), dtype=torch.float32)
     else:
         assert lse.shape == (tokens, heads) and lse.dtype == torch.float32
     if tokens == 0:
         return output, lse
     assert num_pages > 0, "the cache has no pages"
-    prefix_pages, token_lens = _int32(prefix_pages), _int32(token_lens)
-    if block_table.dtype != torch.int32 or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
-        block_table = block_table.to(torch.int32).contiguous()
-    q_nope = q_nope if _tiled(q_nope) else q_nope.contiguous()
-    q_pe = q_pe if _tiled(q_pe) else q_pe.contiguous()
-    assert _tiled(ckv_cache) and _tiled(kpe_cache), \
-        "cache rows must be contiguous, 16-byte aligned and apart, the page stride a multiple of the row stride"
+    if block_table.dtype != torch.int32 or (width > 1 and block_table.stride(1) != 1):
+        block_table = _int32(block_table, "block_table")
+    q_nope, qn_token, qn_head = _tiled(q_nope)
+    q_pe, qp_token, qp_head = _tiled(q_pe)
+    rows_c, c_page, c_row = _tiled(ckv_cache)
+    rows_e, e_page, e_row = _tiled(kpe_cache)
+    assert rows_c is ckv_cache and rows_e is kpe_cache, "cache rows must be contiguous, 16-byte aligned and apart"
     if workspace is None:
-        workspace = _workspace(device, prefix_workspace_size(tokens, heads, device))
-    elif not (workspace.is_cuda and workspace.device == device and workspace.dtype == torch.uint8
-              and workspace.is_contiguous()):
+        workspace = _workspace(index, prefix_workspace_size(tokens, heads, index))
+    elif not (workspace.dtype == torch.uint8 and workspace.is_contiguous()):
         raise ValueError("workspace must be a contiguous uint8 tensor on the inputs' device")
-    _lib.call_on(device, "dsa_shared_prefix_attention", q_nope.data_ptr(), q_nope.stride(0), q_nope.stride(1),
-                 q_pe.data_ptr(), q_pe.stride(0), q_pe.stride(1), ckv_cache.data_ptr(), ckv_cache.stride(0),
-                 ckv_cache.stride(1), kpe_cache.data_ptr(), kpe_cache.stride(0), kpe_cache.stride(1),
+    _lib.call_on(index, "dsa_shared_prefix_attention", q_nope.data_ptr(), qn_token, qn_head, q_pe.data_ptr(), qp_token,
+                 qp_head, ckv_cache.data_ptr(), c_page, c_row, kpe_cache.data_ptr(), e_page, e_row,
                  prefix_pages.data_ptr(), bound, length.data_ptr() if length is not None else None,
-                 block_table.data_ptr(), block_table.stride(0), block_table.shape[0], block_table.shape[1],
+                 block_table.data_ptr(), block_table.stride(0), requests, width,
                  token_request.data_ptr() if token_request is not None else None, token_lens.data_ptr(), tokens,
-                 heads, num_pages, float(sm_scale), output.data_ptr(), output.stride(0), output.stride(1),
+                 heads, num_pages, sm_scale, output.data_ptr(), output.stride(0), output.stride(1),
                  lse.data_ptr(), lse.stride(0), lse.stride(1), workspace.data_ptr(), workspace.numel())
     return output, lse
 
 
-def _tiled(t: torch.Tensor) -> bool:
-    """Whether the TMA can read rows of t [A, B, width] where they are."""
+def _tiled(t: torch.Tensor):
+    """(t, outer, inner stride) of t [A, B, width] if the TMA can read its rows
+    where they are, else of a contiguous copy."""
     outer, inner, last = t.stride()
-    ok = last == 1 and t.data_ptr() % 16 == 0 and inner % 8 == 0 and inner >= t.shape[2]
-    return ok and (t.shape[0] == 1 or (outer >= inner and outer % inner == 0))
+    if last == 1 and inner % 8 == 0 and inner >= t.shape[2] and t.data_ptr() % 16 == 0 and (
+            t.shape[0] == 1 or (outer >= inner and outer % 8 == 0)):
+        return t, outer, inner
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, t.stride(0), t.stride(1)
 
 
-def _int32(t: torch.Tensor) -> torch.Tensor:
-    return t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
+def _int32(t: torch.Tensor, name: str) -> torch.Tensor:
+    if t.dtype == torch.int32 and t.is_contiguous():
+        return t
+    assert t.dtype in (torch.int32, torch.int64), f"{name} must be int32 or int64"
+    return t.to(torch.int32).contiguous()
 
 
 def read_prefix_error(device=None, clear=True) -> int:
     """Synchronise and return the DSA_DEVERR_* bits raised by
     shared_prefix_attention calls that used the device's shared workspace."""
-    device = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
-    index = device.index if device.index is not None else torch.cuda.current_device()
+    index = _index(device)
     bits = 0
     with torch.cuda.device(index):
         stream = torch.cuda.current_stream().cuda_stream

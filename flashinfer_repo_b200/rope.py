@@ -51,13 +51,12 @@ def rope_frequencies(rot_dim, base=10000.0, *, scaling=None, factor=1.0, origina
     return inv.to(device)
 
 
-def _check_rotation(device, positions, inv_freq, tokens, layout):
+def _check_rotation(positions, inv_freq, tokens, layout):
     if layout not in LAYOUTS:
         raise ValueError(f"layout must be one of {sorted(LAYOUTS)}, got {layout!r}")
     assert positions.shape == (tokens,) and positions.dtype in (torch.int32, torch.int64), \
         "positions must be [tokens] int32 or int64"
     assert inv_freq.dim() == 1 and inv_freq.dtype == torch.float64, "inv_freq must be [rot_dim/2] float64"
-    _lib.check_cuda(device, positions=positions, inv_freq=inv_freq)
     return positions.contiguous(), inv_freq.contiguous()
 
 
@@ -74,27 +73,27 @@ def apply_rope(x, positions, inv_freq, *, layout="interleaved", offset=0, invers
     into, x itself for in place; any other overlap with x is not allowed.
     bf16, fp16 or fp32; products in 32 bits, one rounding.
     """
-    assert x.dim() in (2, 3), "x must be [tokens, heads, dim] or [tokens, dim]"
-    assert x.dtype in DTYPES, f"x must be bf16, fp16 or fp32, got {x.dtype}"
-    device, tokens = x.device, x.shape[0]
-    _lib.check_cuda(device, x=x, out=out)
-    positions, inv_freq = _check_rotation(device, positions, inv_freq, tokens, layout)
+    shape = x.shape
+    assert len(shape) in (2, 3), "x must be [tokens, heads, dim] or [tokens, dim]"
+    dtype = DTYPES.get(x.dtype)
+    assert dtype is not None, f"x must be bf16, fp16 or fp32, got {x.dtype}"
+    index = _lib.same_device(x=x, positions=positions, inv_freq=inv_freq, out=out)
+    positions, inv_freq = _check_rotation(positions, inv_freq, shape[0], layout)
     rot = 2 * inv_freq.shape[0]
-    assert 0 <= offset and offset + rot <= x.shape[-1], "the rotated slice reaches past the head"
+    assert 0 <= offset and offset + rot <= shape[-1], "the rotated slice reaches past the head"
+    if x.stride(-1) != 1:
+        assert out is None or out.data_ptr() != x.data_ptr(), "in place needs contiguous heads"
+        x = x.contiguous()
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=device)
-        if x.stride(-1) != 1:
-            x = x.contiguous()
+        out = x.new_empty(shape)
     else:
-        assert out.shape == x.shape and out.dtype == x.dtype and out.stride(-1) == 1
-        if x.stride(-1) != 1:
-            assert out.data_ptr() != x.data_ptr()
-            x = x.contiguous()
-        if out.data_ptr() == x.data_ptr():
-            assert out.stride() == x.stride(), "out shares x's memory with other strides"
-    heads = x.shape[1] if x.dim() == 3 else 1
-    _lib.call_on(device, "dsa_apply_rope", x.data_ptr(), x.stride(0), x.stride(-2) if x.dim() == 3 else 0,
-                 out.data_ptr(), out.stride(0), out.stride(-2) if x.dim() == 3 else 0, DTYPES[x.dtype], tokens,
-                 heads, x.shape[-1], int(offset), rot, positions.data_ptr(), int(positions.dtype == torch.int64),
-                 inv_freq.data_ptr(), LAYOUTS[layout], int(bool(inverse)), float(scale))
+        assert out.shape == shape and out.dtype == x.dtype and out.stride(-1) == 1
+        assert out.data_ptr() != x.data_ptr() or out.stride() == x.stride(), "out shares x's memory with other strides"
+    if len(shape) == 3:
+        heads, x_head, o_head = shape[1], x.stride(1), out.stride(1)
+    else:
+        heads, x_head, o_head = 1, 0, 0
+    _lib.call_on(index, "dsa_apply_rope", x.data_ptr(), x.stride(0), x_head, out.data_ptr(), out.stride(0), o_head,
+                 dtype, shape[0], heads, shape[-1], offset, rot, positions.data_ptr(),
+                 positions.dtype == torch.int64, inv_freq.data_ptr(), LAYOUTS[layout], bool(inverse), scale)
     return out
