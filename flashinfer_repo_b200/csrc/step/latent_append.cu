@@ -18,7 +18,6 @@ struct AppendParams {
   const void* kv;
   int64_t kv_st;
   const void* w;
-  int w_dtype;
   int64_t rows;
   const void* positions;
   int pos64;
@@ -31,18 +30,40 @@ struct AppendParams {
   int* err;
 };
 
-__device__ __forceinline__ float weight(const AppendParams& p, int i) {
-  if (p.w_dtype == DSA_FP32) return static_cast<const float*>(p.w)[i];
-  if (p.w_dtype == DSA_FP16) return to_f32(static_cast<const __half*>(p.w)[i]);
-  return to_f32(static_cast<const __nv_bfloat16*>(p.w)[i]);
+// 8 values from `from` on as they are wanted in the sum: 32 bits.
+template <typename T, bool kVec>
+__device__ __forceinline__ void load8(const T* from, float* v) {
+  if (kVec) {
+#pragma unroll
+    for (int k = 0; k < 8 / Vec<T>::kN; ++k) {
+      const Vec<T> x = reinterpret_cast<const Vec<T>*>(from)[k];
+#pragma unroll
+      for (int i = 0; i < Vec<T>::kN; ++i) v[k * Vec<T>::kN + i] = to_f32(x.v[i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = to_f32(from[i]);
+  }
 }
 
-template <typename T>
+template <typename T, typename W, bool kVec>
 __global__ void __launch_bounds__(256) dsa_latent_append_kernel(const AppendParams p) {
   const int64_t row = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
   const int lane = threadIdx.x & 31;
   if (row >= p.rows) return;
+  // every load of the row is issued before the first is needed
   const int32_t slot = p.slots[row];
+  const T* x = static_cast<const T*>(p.kv) + row * p.kv_st;
+  const W* w = static_cast<const W*>(p.w);
+  const int ia = p.half_layout ? lane : 2 * lane, ib = p.half_layout ? lane + 32 : 2 * lane + 1;
+  float v[2][8], g[2][8];
+  load8<T, kVec>(x + lane * 8, v[0]);
+  load8<T, kVec>(x + 256 + lane * 8, v[1]);
+  const float a = to_f32(x[kLatent + ia]), b = to_f32(x[kLatent + ib]);
+  const int64_t position = load_position(p.positions, p.pos64, row);
+  load8<W, kVec>(w + lane * 8, g[0]);
+  load8<W, kVec>(w + 256 + lane * 8, g[1]);
+  const double freq = p.inv_freq[lane];
   if (slot < 0) {  // a padded row; anything below -1 is a wrong id
     if (slot < -1 && lane == 0) set_error(p.err, kErrBadIndex);
     return;
@@ -52,29 +73,51 @@ __global__ void __launch_bounds__(256) dsa_latent_append_kernel(const AppendPara
     if (lane == 0) set_error(p.err, kErrBadIndex);
     return;
   }
-  const T* x = static_cast<const T*>(p.kv) + row * p.kv_st;
-  float v[16], sum = 0.f;
+  float sum = 0.f;
 #pragma unroll
-  for (int k = 0; k < 16; ++k) {
-    v[k] = to_f32(x[(k >> 3) * 256 + lane * 8 + (k & 7)]);
-    sum += v[k] * v[k];
-  }
+  for (int k = 0; k < 16; ++k) sum += v[k >> 3][k & 7] * v[k >> 3][k & 7];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   const float r = 1.f / sqrtf(sum * (1.f / kLatent) + p.eps);
   __nv_bfloat16* c = p.ckv + page * p.ckv_sp + at * p.ckv_sr;
 #pragma unroll
-  for (int k = 0; k < 16; ++k) {
-    const int i = (k >> 3) * 256 + lane * 8 + (k & 7);
-    c[i] = __float2bfloat16_rn(v[k] * r * weight(p, i));
+  for (int k = 0; k < 2; ++k) {
+    Vec<__nv_bfloat16> y;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y.v[i] = __float2bfloat16_rn(v[k][i] * r * g[k][i]);
+    if (kVec) {
+      *reinterpret_cast<Vec<__nv_bfloat16>*>(c + k * 256 + lane * 8) = y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) c[k * 256 + lane * 8 + i] = y.v[i];
+    }
   }
-  const int ia = p.half_layout ? lane : 2 * lane, ib = p.half_layout ? lane + 32 : 2 * lane + 1;
-  const float a = to_f32(x[kLatent + ia]), b = to_f32(x[kLatent + ib]);
   float cs, sn;
-  rotation(load_position(p.positions, p.pos64, row), p.inv_freq[lane], p.scale, &cs, &sn);
+  rotation(position, freq, p.scale, &cs, &sn);
   __nv_bfloat16* e = p.kpe + page * p.kpe_sp + at * p.kpe_sr;
   e[ia] = __float2bfloat16_rn(a * cs - b * sn);
   e[ib] = __float2bfloat16_rn(b * cs + a * sn);
+}
+
+template <typename T, typename W>
+void launch(const AppendParams& p, cudaStream_t stream) {
+  const unsigned grid = (unsigned)((p.rows * 32 + 255) / 256);
+  // 16-byte accesses where every row, the weights and the latent cache allow them
+  bool vec = p.kv_st % Vec<T>::kN == 0 && p.ckv_sp % 8 == 0 && p.ckv_sr % 8 == 0;
+  for (const void* q : {p.kv, p.w, (const void*)p.ckv}) vec = vec && (reinterpret_cast<uintptr_t>(q) & 15) == 0;
+  if (vec)
+    dsa_latent_append_kernel<T, W, true><<<grid, 256, 0, stream>>>(p);
+  else
+    dsa_latent_append_kernel<T, W, false><<<grid, 256, 0, stream>>>(p);
+}
+template <typename T>
+void launch(const AppendParams& p, int w_dtype, cudaStream_t stream) {
+  if (w_dtype == DSA_BF16)
+    launch<T, __nv_bfloat16>(p, stream);
+  else if (w_dtype == DSA_FP16)
+    launch<T, __half>(p, stream);
+  else
+    launch<T, float>(p, stream);
 }
 
 }  // namespace
@@ -96,13 +139,13 @@ extern "C" int dsa_latent_cache_append(const void* kv, int64_t kv_stride, int kv
     if (t != DSA_BF16 && t != DSA_FP16 && t != DSA_FP32)
       return report_error(DSA_ERR_INVALID_ARG, "unknown element type");
   if (num_tokens == 0) return DSA_OK;
+  if (num_tokens > INT32_MAX) return report_error(DSA_ERR_UNSUPPORTED, "tokens are counted in 32 bits");
   if (!kv || !norm_weight || !positions || !slots || !inv_freq || !ckv_cache || !kpe_cache)
     return report_error(DSA_ERR_INVALID_ARG, "NULL pointer argument");
   AppendParams p;
   p.kv = kv;
   p.kv_st = kv_stride;
   p.w = norm_weight;
-  p.w_dtype = norm_dtype;
   p.rows = num_tokens;
   p.positions = positions;
   p.pos64 = positions_are_64_bit != 0;
@@ -120,13 +163,12 @@ extern "C" int dsa_latent_cache_append(const void* kv, int64_t kv_stride, int kv
   p.half_layout = layout == DSA_ROPE_HALF;
   p.err = device_error;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const unsigned grid = (unsigned)((num_tokens * 32 + 255) / 256);
   if (kv_dtype == DSA_BF16)
-    dsa_latent_append_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(p);
+    launch<__nv_bfloat16>(p, norm_dtype, s);
   else if (kv_dtype == DSA_FP16)
-    dsa_latent_append_kernel<__half><<<grid, 256, 0, s>>>(p);
+    launch<__half>(p, norm_dtype, s);
   else
-    dsa_latent_append_kernel<float><<<grid, 256, 0, s>>>(p);
+    launch<float>(p, norm_dtype, s);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return report_error(DSA_ERR_CUDA, cudaGetErrorString(e));
   return DSA_OK;

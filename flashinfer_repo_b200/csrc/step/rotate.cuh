@@ -18,6 +18,13 @@ __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+// 16 bytes of a tensor, loaded and stored at once.
+template <typename T>
+struct __align__(16) Vec {
+  static constexpr int kN = 16 / sizeof(T);
+  T v[kN];
+};
+
 // cos and sin of position * inv_freq.  The angle is taken in turns in 64 bits
 // and reduced to half a turn before it is rounded to 32 (a 32-bit product is
 // 0.01 rad off at position 1e5): the error is then 2^-25 turns plus 2^-53 of
