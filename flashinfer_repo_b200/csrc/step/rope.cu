@@ -4,20 +4,20 @@
 // is copied.  The inverse turns by the negative angle, which is also the
 // gradient (the rotation's transpose).
 //
-// A CTA takes whole tokens, so that a token's rot/2 angles are computed once
-// and serve all its heads.  Bound by HBM for many rows (each value is read and
-// written once) and by latency for a decode step.  Aligned tensors go by 16
-// bytes a thread and access, four of them in flight while the angles are
-// computed; others value by value.
+// A warp takes a token and a stretch of its heads: its lanes compute the token's
+// rot/2 angles (one each for the usual 64-wide slice) into shared memory, and no
+// barrier of a CTA is in the way.  Bound by HBM for many rows (each value is read
+// and written once) and by latency for a decode step.  Aligned tensors go by 16
+// bytes a lane and access, all of them loaded before the angles are computed;
+// others value by value.
 #include "../../../include/dsa_b200.h"
 #include "rotate.cuh"
 
 namespace dsa {
 namespace {
 
-constexpr int kRopeThreads = 256;
+constexpr int kRopeWarps = 4;
 constexpr int kRopeMaxHalf = 256;  // angles per token (rot <= 512)
-constexpr int kRopeAngles = 1024;  // angles in shared memory
 
 struct RopeParams {
   const void* x;
@@ -28,152 +28,169 @@ struct RopeParams {
   const void* positions;
   int pos64;
   const double* inv_freq;
-  int inverse, tokens_per_cta, per_head;  // per_head: units of a head
-  uint32_t inv_per_head, inv_heads;        // 2^32 / divisor, rounded up
+  int inverse, turned, rest, units, chunks;  // units of a head that turn and that do not, of a token; warps a token
+  uint32_t inv_turned, inv_rest;             // 2^32 / turned, 2^32 / rest, rounded up
   float scale;
 };
 
-__device__ __forceinline__ void angles(const RopeParams& p, int64_t first, int tokens, float* cs, float* sn) {
-  const int half = p.rot / 2;
-  for (int i = threadIdx.x; i < tokens * half; i += kRopeThreads) {
-    const int k = i / half;
+// cos and sin of a token's angles, by the lanes of a warp.
+__device__ __forceinline__ void angles(const RopeParams& p, int64_t token, float* cs, float* sn) {
+  const int64_t position = load_position(p.positions, p.pos64, token);
+  for (int i = threadIdx.x & 31; i < p.rot / 2; i += 32) {
     float c, s;
-    rotation(load_position(p.positions, p.pos64, first + k), p.inv_freq[i - k * half], p.scale, &c, &s);
+    rotation(position, p.inv_freq[i], p.scale, &c, &s);
     cs[i] = c;
     sn[i] = p.inverse ? -s : s;
   }
+  __syncwarp();
 }
 
-// A unit is one access of a head: a 16-byte vector of the rotated slice (kHalf:
-// one of its first half and its partner), or one of the rest, which is copied.
-template <typename T, bool kHalf>
-__global__ void __launch_bounds__(kRopeThreads) dsa_rope_vec_kernel(const RopeParams p) {
-  constexpr int kN = Vec<T>::kN, kUnroll = 4;
-  __shared__ float cs[kRopeAngles], sn[kRopeAngles];
-  const int64_t first = (int64_t)blockIdx.x * p.tokens_per_cta;
-  const int tokens = (int)min((int64_t)p.tokens_per_cta, p.tokens - first);
-  const int half = p.rot / 2, turned = (kHalf ? half : p.rot) / kN;
-  const int units = p.heads * p.per_head, total = tokens * units;
-  const T* x = static_cast<const T*>(p.x) + first * p.x_st;
-  T* o = static_cast<T*>(p.out) + first * p.o_st;
-  for (int e0 = threadIdx.x; e0 - (int)threadIdx.x < total; e0 += kUnroll * kRopeThreads) {
-    Vec<T> a[kUnroll], b[kUnroll];
-    int at[kUnroll], slot[kUnroll], tok[kUnroll], head[kUnroll];
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int e = e0 + u * kRopeThreads;
-      slot[u] = -1;
-      if (e < total) {
-        const int hh = __umulhi(e, p.inv_per_head);  // e / per_head
-        slot[u] = e - hh * p.per_head;
-        tok[u] = __umulhi(hh, p.inv_heads);  // hh / heads
-        head[u] = hh - tok[u] * p.heads;
-        if (slot[u] < turned) {
-          at[u] = p.offset + slot[u] * kN;
-        } else {
-          at[u] = (slot[u] - turned) * kN;
-          if (at[u] >= p.offset) at[u] += p.rot;
-        }
-        const T* src = x + tok[u] * p.x_st + head[u] * p.x_sh + at[u];
-        a[u] = *reinterpret_cast<const Vec<T>*>(src);
-        if (kHalf && slot[u] < turned) b[u] = *reinterpret_cast<const Vec<T>*>(src + half);
-      }
-    }
-    if (e0 == (int)threadIdx.x) {  // the first loads are on their way meanwhile
-      angles(p, first, tokens, cs, sn);
-      __syncthreads();
-    }
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      if (slot[u] < 0) continue;
-      T* dst = o + tok[u] * p.o_st + head[u] * p.o_sh + at[u];
-      if (slot[u] < turned) {
-        const int i0 = tok[u] * half + slot[u] * (kHalf ? kN : kN / 2);
-        if (kHalf) {
-          Vec<T> r;
-#pragma unroll
-          for (int i = 0; i < kN; ++i) {
-            const float c = cs[i0 + i], s = sn[i0 + i], va = to_f32(a[u].v[i]), vb = to_f32(b[u].v[i]);
-            a[u].v[i] = from_f32<T>(va * c - vb * s);
-            r.v[i] = from_f32<T>(vb * c + va * s);
-          }
-          *reinterpret_cast<Vec<T>*>(dst + half) = r;
-        } else {
-#pragma unroll
-          for (int i = 0; i < kN / 2; ++i) {
-            const float c = cs[i0 + i], s = sn[i0 + i], va = to_f32(a[u].v[2 * i]), vb = to_f32(a[u].v[2 * i + 1]);
-            a[u].v[2 * i] = from_f32<T>(va * c - vb * s);
-            a[u].v[2 * i + 1] = from_f32<T>(vb * c + va * s);
-          }
-        }
-      }
-      *reinterpret_cast<Vec<T>*>(dst) = a[u];
-    }
-  }
-}
-
-// Any alignment: a pair of values, or a value of the rest, at a time.
-template <typename T, bool kHalf>
-__global__ void __launch_bounds__(kRopeThreads) dsa_rope_kernel(const RopeParams p) {
-  __shared__ float cs[kRopeAngles], sn[kRopeAngles];
-  const int64_t first = (int64_t)blockIdx.x * p.tokens_per_cta;
-  const int tokens = (int)min((int64_t)p.tokens_per_cta, p.tokens - first);
-  const int half = p.rot / 2;
-  angles(p, first, tokens, cs, sn);
-  __syncthreads();
-  for (int k = 0; k < tokens; ++k) {
-    const T* x = static_cast<const T*>(p.x) + (first + k) * p.x_st;
-    T* o = static_cast<T*>(p.out) + (first + k) * p.o_st;
-    for (int e = threadIdx.x; e < p.heads * half; e += kRopeThreads) {
-      const int h = e / half, i = e - h * half;
-      const int ia = p.offset + (kHalf ? i : 2 * i), ib = kHalf ? ia + half : ia + 1;
-      const float a = to_f32(x[h * p.x_sh + ia]), b = to_f32(x[h * p.x_sh + ib]);
-      const float c = cs[k * half + i], s = sn[k * half + i];
-      o[h * p.o_sh + ia] = from_f32<T>(a * c - b * s);
-      o[h * p.o_sh + ib] = from_f32<T>(b * c + a * s);
-    }
-    if (p.x != p.out) {
-      const int rest = p.dim - p.rot;
-      for (int e = threadIdx.x; e < p.heads * rest; e += kRopeThreads) {
-        const int h = e / rest, r = e - h * rest, d = r < p.offset ? r : r + p.rot;
-        o[h * p.o_sh + d] = x[h * p.x_sh + d];
-      }
-    }
-  }
-}
-
-template <typename T>
-void launch(RopeParams p, int layout, cudaStream_t stream) {
+// A unit is 16 bytes of a head.  The units that turn come first, of all heads:
+// mixed in a warp with the others, which are copied, they would keep its lanes
+// waiting.  In the half layout the partner of a unit is rot/2 values away, in
+// another lane: the lanes of a head swap their units by shuffles, so that loads
+// and stores stay whole lines (a lane that loads both its halves itself moves
+// half lines: 33-46 instead of 26 us for 134 MB of bf16, half of it turned).
+template <typename T, bool kHalf, int kUnits>
+__global__ void __launch_bounds__(32 * kRopeWarps) dsa_rope_vec_kernel(const RopeParams p) {
   constexpr int kN = Vec<T>::kN;
-  const bool half = layout == DSA_ROPE_HALF;
-  const int turned = half ? p.rot / 2 : p.rot;
-  bool vec = turned % kN == 0 && p.offset % kN == 0 && p.dim % kN == 0;
+  __shared__ __align__(16) float cs_all[kRopeWarps][kRopeMaxHalf], sn_all[kRopeWarps][kRopeMaxHalf];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t task = (int64_t)blockIdx.x * kRopeWarps + warp, token = task / p.chunks;
+  if (token >= p.tokens) return;
+  float *cs = cs_all[warp], *sn = sn_all[warp];
+  const int turning = p.heads * p.turned;
+  const int first = (int)(task - token * p.chunks) * (32 * kUnits) + lane;
+  const T* x = static_cast<const T*>(p.x) + token * p.x_st;
+  T* o = static_cast<T*>(p.out) + token * p.o_st;
+  Vec<T> a[kUnits];
+  auto place = [&](int e, int* head, int* slot) -> int {  // first value of the unit in its head
+    if (e < turning) {
+      *head = p.turned == 1 ? e : __umulhi(e, p.inv_turned);
+      *slot = e - *head * p.turned;
+      return p.offset + *slot * kN;
+    }
+    e -= turning;
+    *head = p.rest == 1 ? e : __umulhi(e, p.inv_rest);
+    const int at = (e - *head * p.rest) * kN;
+    return at < p.offset ? at : at + p.rot;
+  };
+#pragma unroll
+  for (int u = 0; u < kUnits; ++u) {
+    const int e = first + 32 * u;
+    if (e < p.units) {
+      int head, slot;
+      const int at = place(e, &head, &slot);
+      a[u] = *reinterpret_cast<const Vec<T>*>(x + head * p.x_sh + at);
+    }
+  }
+  angles(p, token, cs, sn);
+#pragma unroll
+  for (int u = 0; u < kUnits; ++u) {
+    const int e = first + 32 * u;
+    Vec<T> other;
+    if (kHalf) {  // a head's lanes lie side by side: turned is a power of two up to 32
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        reinterpret_cast<uint32_t*>(&other)[i] =
+            __shfl_xor_sync(0xffffffffu, reinterpret_cast<const uint32_t*>(&a[u])[i], p.turned >> 1);
+    }
+    if (e >= p.units) continue;
+    int head, slot;
+    const int at = place(e, &head, &slot);
+    if (e < turning) {
+      constexpr int kA = kHalf ? kN : kN / 2, kQ = kA < 4 ? kA : 4;  // angles of the unit, of a shared load
+      struct __align__(4 * kQ) Angles {
+        float v[kQ];
+      };
+      const bool second = kHalf && slot >= p.turned / 2;
+      const int i0 = (second ? slot - p.turned / 2 : slot) * kA;
+#pragma unroll
+      for (int q = 0; q < kA; q += kQ) {
+        const Angles c = *reinterpret_cast<const Angles*>(cs + i0 + q);
+        const Angles s = *reinterpret_cast<const Angles*>(sn + i0 + q);
+#pragma unroll
+        for (int i = 0; i < kQ; ++i) {
+          if (kHalf) {
+            const float mine = to_f32(a[u].v[q + i]), its = to_f32(other.v[q + i]);
+            a[u].v[q + i] = from_f32<T>(mine * c.v[i] + its * (second ? s.v[i] : -s.v[i]));
+          } else {
+            const float va = to_f32(a[u].v[2 * (q + i)]), vb = to_f32(a[u].v[2 * (q + i) + 1]);
+            a[u].v[2 * (q + i)] = from_f32<T>(va * c.v[i] - vb * s.v[i]);
+            a[u].v[2 * (q + i) + 1] = from_f32<T>(vb * c.v[i] + va * s.v[i]);
+          }
+        }
+      }
+    }
+    *reinterpret_cast<Vec<T>*>(o + head * p.o_sh + at) = a[u];
+  }
+}
+
+// Any alignment: a warp per token, a pair of values or a value of the rest at a time.
+template <typename T, bool kHalf>
+__global__ void __launch_bounds__(32 * kRopeWarps) dsa_rope_kernel(const RopeParams p) {
+  __shared__ float cs_all[kRopeWarps][kRopeMaxHalf], sn_all[kRopeWarps][kRopeMaxHalf];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t token = (int64_t)blockIdx.x * kRopeWarps + warp;
+  if (token >= p.tokens) return;
+  float *cs = cs_all[warp], *sn = sn_all[warp];
+  const int half = p.rot / 2;
+  angles(p, token, cs, sn);
+  const T* x = static_cast<const T*>(p.x) + token * p.x_st;
+  T* o = static_cast<T*>(p.out) + token * p.o_st;
+  for (int e = lane; e < p.heads * half; e += 32) {
+    const int h = e / half, i = e - h * half;
+    const int ia = p.offset + (kHalf ? i : 2 * i), ib = kHalf ? ia + half : ia + 1;
+    const float a = to_f32(x[h * p.x_sh + ia]), b = to_f32(x[h * p.x_sh + ib]);
+    o[h * p.o_sh + ia] = from_f32<T>(a * cs[i] - b * sn[i]);
+    o[h * p.o_sh + ib] = from_f32<T>(b * cs[i] + a * sn[i]);
+  }
+  if (p.x != p.out) {
+    const int rest = p.dim - p.rot;
+    for (int e = lane; e < p.heads * rest; e += 32) {
+      const int h = e / rest, r = e - h * rest, d = r < p.offset ? r : r + p.rot;
+      o[h * p.o_sh + d] = x[h * p.x_sh + d];
+    }
+  }
+}
+
+template <typename T, bool kHalf>
+void launch(RopeParams p, cudaStream_t stream) {
+  constexpr int kN = Vec<T>::kN, kMany = 4;
+  p.turned = p.rot / kN;
+  p.rest = p.x == p.out ? 0 : (p.dim - p.rot) / kN;
+  const int64_t units = (int64_t)p.heads * (p.turned + p.rest), widest = p.turned > p.rest ? p.turned : p.rest;
+  // the divisions by multiplication are exact while numerator * divisor < 2^32
+  bool vec = p.rot % kN == 0 && p.offset % kN == 0 && p.dim % kN == 0 && units * widest < (1LL << 32);
+  if (kHalf) vec = vec && p.turned >= 2 && p.turned <= 32 && (p.turned & (p.turned - 1)) == 0;
   for (int64_t s : {p.x_st, p.x_sh, p.o_st, p.o_sh}) vec = vec && s % kN == 0;
   for (const void* q : {p.x, (const void*)p.out}) vec = vec && (reinterpret_cast<uintptr_t>(q) & 15) == 0;
-  p.per_head = turned / kN + (p.x == p.out ? 0 : (p.dim - p.rot) / kN);
-  // tokens of a CTA: four units a thread, but one CTA at least for every SM, and
-  // the angles in shared memory
-  const int64_t units = (int64_t)p.heads * (p.per_head < 1 ? 1 : p.per_head), angles = kRopeAngles / (p.rot / 2);
-  int64_t per_cta = 4 * kRopeThreads / units;
-  per_cta = per_cta < p.tokens / 148 ? per_cta : p.tokens / 148;
-  per_cta = per_cta < angles ? per_cta : angles;
-  p.tokens_per_cta = (int)(per_cta < 1 ? 1 : per_cta);
-  // the divisions by multiplication are exact while numerator * divisor < 2^32
-  const int64_t top = units * p.tokens_per_cta;
-  vec = vec && top * p.per_head < (1LL << 32) && top / (p.per_head < 1 ? 1 : p.per_head) * p.heads < (1LL << 32);
-  const unsigned grid = (unsigned)((p.tokens + p.tokens_per_cta - 1) / p.tokens_per_cta);
   if (vec) {
-    p.inv_per_head = (uint32_t)(((1ULL << 32) + p.per_head - 1) / p.per_head);
-    p.inv_heads = (uint32_t)(((1ULL << 32) + p.heads - 1) / p.heads);
-    if (half)
-      dsa_rope_vec_kernel<T, true><<<grid, kRopeThreads, 0, stream>>>(p);
+    p.units = (int)units;
+    p.inv_turned = (uint32_t)(((1ULL << 32) + p.turned - 1) / p.turned);
+    p.inv_rest = p.rest ? (uint32_t)(((1ULL << 32) + p.rest - 1) / p.rest) : 0;
+    // four units a lane keep enough bytes in flight (197 MB of fp32: 32 us, 44
+    // with one); where that leaves SMs without a CTA, one unit a lane is sooner
+    // done (64 tokens of 16 heads: 2.1 us, 3.2 with four)
+    auto grid = [&](int per_lane) {
+      p.chunks = (p.units + 32 * per_lane - 1) / (32 * per_lane);
+      return (unsigned)((p.tokens * p.chunks + kRopeWarps - 1) / kRopeWarps);
+    };
+    const unsigned ctas = grid(kMany);
+    if (ctas >= 148)
+      dsa_rope_vec_kernel<T, kHalf, kMany><<<ctas, 32 * kRopeWarps, 0, stream>>>(p);
     else
-      dsa_rope_vec_kernel<T, false><<<grid, kRopeThreads, 0, stream>>>(p);
-  } else if (half) {
-    dsa_rope_kernel<T, true><<<grid, kRopeThreads, 0, stream>>>(p);
+      dsa_rope_vec_kernel<T, kHalf, 1><<<grid(1), 32 * kRopeWarps, 0, stream>>>(p);
   } else {
-    dsa_rope_kernel<T, false><<<grid, kRopeThreads, 0, stream>>>(p);
+    dsa_rope_kernel<T, kHalf><<<(unsigned)((p.tokens + kRopeWarps - 1) / kRopeWarps), 32 * kRopeWarps, 0, stream>>>(p);
   }
+}
+template <typename T>
+void launch(const RopeParams& p, int layout, cudaStream_t stream) {
+  if (layout == DSA_ROPE_HALF)
+    launch<T, true>(p, stream);
+  else
+    launch<T, false>(p, stream);
 }
 
 }  // namespace
