@@ -13,6 +13,20 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 
+// Two 32-bit operations at once.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(d)
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
+  return reinterpret_cast<float2&>(d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return reinterpret_cast<float2&>(d);
+}
+
 // Barrier among nthreads that tells all of them whether every one brought true.
 __device__ __forceinline__ bool named_bar_all(int id, int nthreads, bool mine) {
   uint32_t all;

@@ -50,7 +50,8 @@ struct PrefixParams {
   int max_prefix, batch, max_own, num_pages;  // max_own: rows that a row of the block table has room for
   int groups, blocks, group_per_token, max_pairs;
   int q_boxes;  // query loads of 64 rows
-  float scale_log2;
+  float scale_log2;  // above zero
+  int negate;        // sm_scale is below zero
   __nv_bfloat16* out;
   int64_t out_st, out_sh;
   float* lse;
@@ -79,15 +80,22 @@ __device__ __forceinline__ int tokens_of(const PrefixParams& p, int block) {
   const unsigned last = min((unsigned)(block + 1) * kGroups, (unsigned)p.groups) - 1;
   return (int)(last / (unsigned)p.group_per_token) - first_token(p, block) + 1;
 }
-// The pairs that work: one tile each at least.  Tile u of the U tiles belongs
-// to the pair c with start(c) <= u < start(c + 1).
-__device__ __forceinline__ int pairs_used(const PrefixParams& p, long long tiles) {
-  return (int)min((long long)p.max_pairs, tiles);
-}
-__device__ __forceinline__ long long pair_start(long long tiles, int pairs, int c) { return tiles * c / pairs; }
-__device__ __forceinline__ int pair_of(long long tiles, int pairs, long long u) {
-  return (int)(((u + 1) * pairs - 1) / tiles);
-}
+// The tiles are dealt out in stretches of `each`, one more for the first `more`
+// pairs; with fewer tiles than pairs some pairs stay idle.
+struct Deal {
+  long long each;
+  int more, pairs;
+  __device__ __forceinline__ Deal(const PrefixParams& p, long long tiles) {
+    pairs = (int)min((long long)p.max_pairs, tiles);
+    each = tiles < (1LL << 31) ? (long long)((unsigned)tiles / (unsigned)pairs) : tiles / pairs;
+    more = (int)(tiles - each * pairs);
+  }
+  __device__ __forceinline__ long long start(int pair) const { return each * pair + min(pair, more); }
+  __device__ __forceinline__ int pair_of(long long tile) const {
+    const long long longer = (each + 1) * more;
+    return tile < longer ? (int)(tile / (each + 1)) : more + (int)((tile - longer) / each);
+  }
+};
 
 // Tiles of a row block's page list: the prefix, then for every run of tokens of
 // the same request the pages that all of them see whole, once, and for every
@@ -166,6 +174,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)cluster_ctarank(), pair = blockIdx.x >> 1;
 
+  if (threadIdx.x == 32)
+    for (const CUtensorMap* m : {&map_qn, &map_qp, &map_ckv3, &map_ckv2, &map_kpe})
+      asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
   if (threadIdx.x == 0) {
     mbar_init(&S.q_full, 2);
     mbar_init(&S.q_empty, 1);
@@ -210,13 +221,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   __syncthreads();
   before -= mine;
   long long tiles = 0;
+#pragma unroll
   for (int w = 0; w < kThreads / 32; ++w) {
     if (w < warp) before += S.sums[w];
     tiles += S.sums[w];
   }
-  const int pairs = pairs_used(p, tiles);
-  const long long u0 = pair < pairs ? pair_start(tiles, pairs, pair) : tiles;
-  const long long u1 = pair < pairs ? pair_start(tiles, pairs, pair + 1) : tiles;
+  const Deal deal(p, tiles);
+  const long long u0 = pair < deal.pairs ? deal.start(pair) : tiles, u1 = pair < deal.pairs ? deal.start(pair + 1) : tiles;
   if (blockIdx.x == 0 || (before <= u0 && u0 < before + mine)) {
     long long c = before;
     for (int b = b0; b < b1; ++b) {
@@ -269,8 +280,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const uint32_t firsts = __ballot_sync(0xffffffffu, first);
       const int run = __popc(firsts & (0xffffffffu >> (31 - lane)));
       int least = len;
-      uint32_t run_sees = 0;
-      for (int i = 0; i < kGroups; ++i) {
+      uint32_t run_sees = sees;
+      for (int i = 0; i < kGroups && __popc(firsts) < nt; ++i) {  // some run is longer than one token
         const int r = __shfl_sync(0xffffffffu, run, i), l = __shfl_sync(0xffffffffu, len, i);
         const uint32_t m = __shfl_sync(0xffffffffu, sees, i);
         if (i < nt && r == run) {
@@ -559,47 +570,57 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const bool live = group < p.groups;
       const int token = live ? (unsigned)group / (unsigned)p.group_per_token : 0;
       const int my_bit = rank * 4 + (row >> 4);
-      float m = -INFINITY, l = 0.f;
+      float m = -INFINITY;
+      float2 sums = make_float2(0.f, 0.f);
       int span = 0;
       for (int i = 0; i < count; ++i, ++it) {
         const int k = 2 * (g.tile0 + i) + page;
         ok = ok && mbar_wait(&S.valid_full[it & 3], (it >> 2) & 1) && mbar_wait_cluster(&S.s_full[it & 1], (it >> 1) & 1);
         tc_fence_after();
-        bool sees = live;
+        bool sees = true;  // rows behind the last token see all: their queries are zeros and nobody reads them
         if (k >= g.pre_pages && k < g.pages) {
           span = span_of(g, k, span);
-          sees = live && ((g.sees[span] >> my_bit) & 1);
+          sees = (g.sees[span] >> my_bit) & 1;
         }
         // the page's rows are at the end of its 64 columns
         const int from = sees ? 64 - S.valid[it & 3][page] - 32 * half : 32;
-        float x[32];
-        tmem_ld32(lanes + kTmemS + 64 * (it & 1) + 32 * half, x);
+        float2 x[16];
+        tmem_ld32(lanes + kTmemS + 64 * (it & 1) + 32 * half, reinterpret_cast<float*>(x));
+        if (p.negate) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) x[j] = make_float2(-x[j].x, -x[j].y);
+        }
+        if (!__all_sync(0xffffffffu, from <= 0)) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            if (2 * j < from) x[j].x = -INFINITY;
+            if (2 * j + 1 < from) x[j].y = -INFINITY;
+          }
+        }
         float top = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          x[j] = j >= from ? x[j] * p.scale_log2 : -INFINITY;
-          top = fmaxf(top, x[j]);
-        }
+        for (int j = 0; j < 16; ++j) top = fmaxf(top, fmaxf(x[j].x, x[j].y));
         S.red[it & 1][page * 2 + half][row] = top;
         if (!(ok = named_bar_all(1, kSoftmaxThreads, ok))) break;
-        top = fmaxf(fmaxf(S.red[it & 1][0][row], S.red[it & 1][1][row]),
-                    fmaxf(S.red[it & 1][2][row], S.red[it & 1][3][row]));
+        top = p.scale_log2 * fmaxf(fmaxf(S.red[it & 1][0][row], S.red[it & 1][1][row]),
+                                   fmaxf(S.red[it & 1][2][row], S.red[it & 1][3][row]));
         // the maximum moves on a rise of more than 2^kLazy only (weights up to
         // 2^8 lose nothing in 32 bits), so O is rescaled on few tiles
         float alpha = 1.f;
         if (top > m + kLazy || m == -INFINITY) {
           alpha = m == -INFINITY ? 1.f : ex2_approx(m - top);
           m = top;
-          l *= alpha;
+          sums = make_float2(sums.x * alpha, sums.y * alpha);
         }
-        const float sub = m == -INFINITY ? 0.f : m;
+        const float sub = m == -INFINITY ? 0.f : -m;
         uint32_t w[16];
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           // weights are rounded to bf16 for the matrix product, the sum takes them as they are
-          const float a = ex2_approx(x[2 * j] - sub), b = ex2_approx(x[2 * j + 1] - sub);
-          l += a + b;
-          w[j] = pack_bf16(a, b);
+          float2 e = fma2(x[j], make_float2(p.scale_log2, p.scale_log2), make_float2(sub, sub));
+          e = make_float2(ex2_approx(e.x), ex2_approx(e.y));
+          sums = add2(sums, e);
+          w[j] = pack_bf16(e.x, e.y);
         }
 #pragma unroll
         for (int j = 0; j < 16; ++j) asm volatile("" : "+r"(w[j]));  // done before the wait, not behind it
@@ -634,6 +655,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
       if (!ok) break;
       // the four threads of a row add up their sums; O is complete
+      float l = sums.x + sums.y;
       S.red[it & 1][page * 2 + half][row] = l;
       ok = mbar_wait_cluster(&S.pv_done, (it - 1) & 1);
       if (!(ok = named_bar_all(1, kSoftmaxThreads, ok))) break;
@@ -685,6 +707,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     tc_fence_after();
     tmem_dealloc_pair(tmem, 512);
   }
+  // here and not at the start: 13.4 against 14.6 us for the smallest call, no
+  // difference beyond 1% for the others
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
@@ -701,12 +725,12 @@ __global__ void __launch_bounds__(kMergeRows * kMergeQuads)
     dsa_prefix_merge_kernel(const PrefixParams p, const int by_cut) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const long long tiles = p.cum[p.blocks];
-  const int pairs = pairs_used(p, tiles);
+  const Deal deal(p, tiles);
   int lo = blockIdx.y;
   if (by_cut) {
     const int cut = blockIdx.y + 1;
-    if (cut >= pairs) return;
-    const long long at = pair_start(tiles, pairs, cut);
+    if (cut >= deal.pairs) return;
+    const long long at = deal.start(cut);
     int hi = p.blocks;
     lo = 0;
     while (hi - lo > 1) {
@@ -716,9 +740,9 @@ __global__ void __launch_bounds__(kMergeRows * kMergeQuads)
       else
         hi = mid;
     }
-    if (at == p.cum[lo] || pair_start(tiles, pairs, cut - 1) > p.cum[lo]) return;  // no cut inside, or not the first
+    if (at == p.cum[lo] || deal.start(cut - 1) > p.cum[lo]) return;  // no cut inside, or not the first
   }
-  const int first = pair_of(tiles, pairs, p.cum[lo]), last = pair_of(tiles, pairs, p.cum[lo + 1] - 1);
+  const int first = deal.pair_of(p.cum[lo]), last = deal.pair_of(p.cum[lo + 1] - 1);
   if (first == last) return;  // one pair had it all and wrote the results
   const int row = blockIdx.x / (128 / kMergeQuads) * kMergeRows + threadIdx.x % kMergeRows;
   const int quad = blockIdx.x % (128 / kMergeQuads) * kMergeQuads + threadIdx.x / kMergeRows;
@@ -948,7 +972,11 @@ extern "C" int dsa_shared_prefix_attention(
   p.blocks = (int)w.blocks;
   p.max_pairs = pairs;
   p.q_boxes = q_boxes;
-  p.scale_log2 = sm_scale * 1.44269504088896340736f;
+  // scores are scaled after the maximum is taken: a scale below zero turns them
+  // over first, and zero becomes a scale that makes every score nothing
+  const float scale = sm_scale * 1.44269504088896340736f;
+  p.negate = scale < 0.f;
+  p.scale_log2 = scale == 0.f ? 1e-30f : p.negate ? -scale : scale;
   p.out = static_cast<__nv_bfloat16*>(output);
   p.out_st = out_stride_token;
   p.out_sh = out_stride_head;
