@@ -57,7 +57,10 @@ struct PrefixParams {
   float* lse;
   int64_t lse_st, lse_sh;
   int* err;
-  long long* cum;  // [blocks + 1] tiles before each row block, for the merge grid
+  // for the merge grid: tiles before each row block [blocks + 1] and the row
+  // block in which each pair begins [max_pairs]
+  long long* cum;
+  int* begins;
   float* parts;    // [blocks + max_pairs] partials
 };
 
@@ -242,6 +245,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     if (blockIdx.x == 0 && b1 == p.blocks) p.cum[p.blocks] = tiles;
   }
   __syncthreads();
+  if (threadIdx.x == 0 && rank == 0 && u0 < u1) p.begins[pair] = S.block;
 
   if (warp == 11) {
     // ------------------------------------------------------------- segments
@@ -715,55 +719,51 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 // ----------------------------------------------------------------- merge
 // Rows whose block several pairs share: with partials (O_k, m_k, l_k),
 //   o = sum_k 2^(m_k - M) O_k / sum_k 2^(m_k - M) l_k.
-// A CTA takes 8 rows of a row block and 32 of its 128 column quads: thread i the
-// row i % 8, so that 8 rows of a quad are read as one line.
-// The grid has a slice for every row block or, where those are more, for every
-// boundary between pairs: then the row block whose first cut the boundary is.
-constexpr int kMergeRows = 8, kMergeQuads = 32;  // rows and column quads of a CTA
+// A CTA takes 8 rows of a row block and 32 kQuads of its 128 column quads: thread
+// i the row i % 8, so that 8 rows of a quad are read as one line.  The grid has a
+// slice for every row block or, where those are more, for every boundary between
+// pairs: then the row block whose first cut the boundary is.
+constexpr int kMergeRows = 8, kMergeColumns = 32;
 
-__global__ void __launch_bounds__(kMergeRows * kMergeQuads)
+template <int kQuads, int kAhead>  // kAhead: partials whose loads are in flight together
+__global__ void __launch_bounds__(kMergeRows * kMergeColumns)
     dsa_prefix_merge_kernel(const PrefixParams p, const int by_cut) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const long long tiles = p.cum[p.blocks];
-  const Deal deal(p, tiles);
+  const int cut = blockIdx.y + 1;
   int lo = blockIdx.y;
-  if (by_cut) {
-    const int cut = blockIdx.y + 1;
-    if (cut >= deal.pairs) return;
-    const long long at = deal.start(cut);
-    int hi = p.blocks;
-    lo = 0;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (p.cum[mid] <= at)
-        lo = mid;
-      else
-        hi = mid;
-    }
-    if (at == p.cum[lo] || deal.start(cut - 1) > p.cum[lo]) return;  // no cut inside, or not the first
-  }
-  const int first = deal.pair_of(p.cum[lo]), last = deal.pair_of(p.cum[lo + 1] - 1);
+  if (by_cut) lo = p.begins[cut];  // tiles >= blocks >= pairs here: every pair works
+  const Deal deal(p, tiles);
+  const long long c0 = p.cum[lo], c1 = p.cum[lo + 1];
+  // a cut on the block's edge is none, and a block is joined once, at its first
+  if (by_cut && (deal.start(cut) == c0 || deal.start(cut - 1) > c0)) return;
+  const int first = deal.pair_of(c0), last = deal.pair_of(c1 - 1);
   if (first == last) return;  // one pair had it all and wrote the results
-  const int row = blockIdx.x / (128 / kMergeQuads) * kMergeRows + threadIdx.x % kMergeRows;
-  const int quad = blockIdx.x % (128 / kMergeQuads) * kMergeQuads + threadIdx.x / kMergeRows;
+  constexpr int kParts = 128 / (kMergeColumns * kQuads);
+  const int row = blockIdx.x / kParts * kMergeRows + threadIdx.x % kMergeRows;
+  const int quad = blockIdx.x % kParts * (kMergeColumns * kQuads) + threadIdx.x / kMergeRows;
   const int group = lo * kGroups + (row >> 4);
   if (group >= p.groups) return;
   float m = -INFINITY, l = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  constexpr int kAhead = 8;  // partials whose loads are in flight together
+  float4 o[kQuads];
+#pragma unroll
+  for (int j = 0; j < kQuads; ++j) o[j] = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int k0 = first; k0 <= last; k0 += kAhead) {
     float mk[kAhead], lk[kAhead];
-    float4 v[kAhead];
+    float4 v[kAhead][kQuads];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       mk[i] = -INFINITY;
       lk[i] = 0.f;
-      v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int j = 0; j < kQuads; ++j) v[i][j] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (k0 + i <= last) {
         const float* part = p.parts + (int64_t)(lo + k0 + i) * kSlotFloats;
         mk[i] = __ldcg(part + 2 * kRows * 512 + row);
         lk[i] = __ldcg(part + 2 * kRows * 512 + 2 * kRows + row);
-        v[i] = __ldcg(reinterpret_cast<const float4*>(part) + quad * (2 * kRows) + row);
+#pragma unroll
+        for (int j = 0; j < kQuads; ++j)
+          v[i][j] = __ldcg(reinterpret_cast<const float4*>(part) + (quad + kMergeColumns * j) * (2 * kRows) + row);
       }
     }
     float top = m;
@@ -772,22 +772,28 @@ __global__ void __launch_bounds__(kMergeRows * kMergeQuads)
     const float a = m == -INFINITY ? 0.f : exp2f(m - top);
     m = top;
     l *= a;
-    o = make_float4(o.x * a, o.y * a, o.z * a, o.w * a);
+#pragma unroll
+    for (int j = 0; j < kQuads; ++j) o[j] = make_float4(o[j].x * a, o[j].y * a, o[j].z * a, o[j].w * a);
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       const float b = mk[i] == -INFINITY ? 0.f : exp2f(mk[i] - top);
       l += lk[i] * b;
-      o.x += v[i].x * b;
-      o.y += v[i].y * b;
-      o.z += v[i].z * b;
-      o.w += v[i].w * b;
+#pragma unroll
+      for (int j = 0; j < kQuads; ++j) {
+        o[j].x += v[i][j].x * b;
+        o[j].y += v[i][j].y * b;
+        o[j].z += v[i][j].z * b;
+        o[j].w += v[i][j].w * b;
+      }
     }
   }
   const int token = (unsigned)group / (unsigned)p.group_per_token;
   const int head = (group - token * p.group_per_token) * 16 + (row & 15);
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  *reinterpret_cast<uint2*>(p.out + token * p.out_st + head * p.out_sh + quad * 4) =
-      make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+#pragma unroll
+  for (int j = 0; j < kQuads; ++j)
+    *reinterpret_cast<uint2*>(p.out + token * p.out_st + head * p.out_sh + (quad + kMergeColumns * j) * 4) =
+        make_uint2(pack_bf16(o[j].x * inv, o[j].y * inv), pack_bf16(o[j].z * inv, o[j].w * inv));
   if (quad == 0) p.lse[token * p.lse_st + head * p.lse_sh] = l == 0.f ? -INFINITY : m + log2f(l);
 }
 
@@ -848,14 +854,15 @@ int resident_pairs() {
 }
 
 struct Layout {
-  int64_t blocks, cum, parts;
+  int64_t blocks, cum, begins, parts;
   size_t bytes;
 };
 Layout workspace_layout(int64_t tokens, int64_t heads, int pairs) {
   Layout w;
   w.blocks = (tokens * (heads / 16) + kGroups - 1) / kGroups;
   w.cum = 256;
-  w.parts = w.cum + ((w.blocks + 1) * 8 + 255) / 256 * 256;
+  w.begins = w.cum + (w.blocks + 1) * 8;
+  w.parts = (w.begins + pairs * 4 + 255) / 256 * 256;
   // a row block that one pair finishes needs no partial, but has a number
   w.bytes = (size_t)(w.parts + (w.blocks + pairs) * (int64_t)kSlotFloats * 4);
   return w;
@@ -985,15 +992,19 @@ extern "C" int dsa_shared_prefix_attention(
   p.lse_sh = lse_stride_head;
   p.err = static_cast<int*>(workspace);
   p.cum = reinterpret_cast<long long*>(static_cast<char*>(workspace) + w.cum);
+  p.begins = reinterpret_cast<int*>(static_cast<char*>(workspace) + w.begins);
   p.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + w.parts);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e = launch_after(dsa_prefix_attention_kernel, dim3(2 * pairs), kThreads, sizeof(PairSmem), s, map_qn, map_qp,
                                map_ckv3, map_ckv2, map_kpe, p);
   if (e == cudaSuccess && pairs > 1) {
     const int rows = (p.groups < kGroups ? p.groups : kGroups) * 16, by_cut = p.blocks >= pairs;
-    e = launch_after(dsa_prefix_merge_kernel,
-                     dim3(rows / kMergeRows * (128 / kMergeQuads), (unsigned)(by_cut ? pairs - 1 : p.blocks)),
-                     kMergeRows * kMergeQuads, 0, s, p, by_cut);
+    const unsigned x = rows / kMergeRows, y = (unsigned)(by_cut ? pairs - 1 : p.blocks), threads = kMergeRows * kMergeColumns;
+    // few row blocks have many partials each: more threads, each with more of them in flight
+    if (x * y <= 148)
+      e = launch_after(dsa_prefix_merge_kernel<1, 8>, dim3(4 * x, y), threads, 0, s, p, by_cut);
+    else
+      e = launch_after(dsa_prefix_merge_kernel<4, 2>, dim3(x, y), threads, 0, s, p, by_cut);
   }
   if (e != cudaSuccess) return report_error(DSA_ERR_CUDA, cudaGetErrorString(e));
   return DSA_OK;
