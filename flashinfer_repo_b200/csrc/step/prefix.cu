@@ -61,7 +61,9 @@ struct PrefixParams {
   // block in which each pair begins [max_pairs]
   long long* cum;
   int* begins;
-  float* parts;    // [blocks + max_pairs] partials
+  // partials, two a pair: of the stretch's first row block and, where that is
+  // another one, of its last; those between are the pair's alone
+  float* parts;
 };
 
 __device__ __forceinline__ int prefix_rows(const PrefixParams& p) {
@@ -133,7 +135,7 @@ __device__ int tiles_of(const PrefixParams& p, int block, int pre_pages) {
 // One pair's stretch of a row block's pages.  Span 2 i: the pages that the run of
 // tokens beginning with token i shares, span 2 i + 1: the other pages of token i.
 struct Segment {
-  int block, tile0, count, whole;  // whole: no other pair works on the row block
+  int block, tile0, count, whole, slot;  // whole: no other pair works on the row block; slot of the partial otherwise
   int pre_pages, pre_rows, pages;
   int end[2 * kGroups], from[2 * kGroups];      // last page + 1 in the list, first page of the request
   int request[2 * kGroups], rows[2 * kGroups];  // rows of the request that the span's tokens see
@@ -323,6 +325,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         g.pre_rows = pre;
         g.pages = pages;
         g.whole = u == c0 && c1 <= u1;
+        g.slot = 2 * pair + (n > 0);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&S.seg_full[s]);
@@ -668,7 +671,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       named_bar_sync(1, kSoftmaxThreads);  // red is written again by the next tile
       const int head = live ? (group - token * p.group_per_token) * 16 + (row & 15) : 0;
       const int dv = half * 256 + page * 128;  // the 128 columns of O in these lanes
-      float* part = p.parts + (int64_t)(g.block + pair) * kSlotFloats;
+      float* part = p.parts + (int64_t)g.slot * kSlotFloats;
       const bool whole = g.whole;
       const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
@@ -739,6 +742,7 @@ __global__ void __launch_bounds__(kMergeRows * kMergeColumns)
   if (by_cut && (deal.start(cut) == c0 || deal.start(cut - 1) > c0)) return;
   const int first = deal.pair_of(c0), last = deal.pair_of(c1 - 1);
   if (first == last) return;  // one pair had it all and wrote the results
+  const bool began_before = deal.start(first) < c0;
   constexpr int kParts = 128 / (kMergeColumns * kQuads);
   const int row = blockIdx.x / kParts * kMergeRows + threadIdx.x % kMergeRows;
   const int quad = blockIdx.x % kParts * (kMergeColumns * kQuads) + threadIdx.x / kMergeRows;
@@ -758,7 +762,9 @@ __global__ void __launch_bounds__(kMergeRows * kMergeColumns)
 #pragma unroll
       for (int j = 0; j < kQuads; ++j) v[i][j] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (k0 + i <= last) {
-        const float* part = p.parts + (int64_t)(lo + k0 + i) * kSlotFloats;
+        // a pair that began before the block has it as its last, any other as its first
+        const int slot = 2 * (k0 + i) + (k0 + i == first && began_before);
+        const float* part = p.parts + (int64_t)slot * kSlotFloats;
         mk[i] = __ldcg(part + 2 * kRows * 512 + row);
         lk[i] = __ldcg(part + 2 * kRows * 512 + 2 * kRows + row);
 #pragma unroll
@@ -863,8 +869,7 @@ Layout workspace_layout(int64_t tokens, int64_t heads, int pairs) {
   w.cum = 256;
   w.begins = w.cum + (w.blocks + 1) * 8;
   w.parts = (w.begins + pairs * 4 + 255) / 256 * 256;
-  // a row block that one pair finishes needs no partial, but has a number
-  w.bytes = (size_t)(w.parts + (w.blocks + pairs) * (int64_t)kSlotFloats * 4);
+  w.bytes = (size_t)(w.parts + 2 * pairs * (int64_t)kSlotFloats * 4);
   return w;
 }
 

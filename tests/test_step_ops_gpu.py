@@ -351,6 +351,54 @@ def test_prefix_long_and_batched():
     assert fi.read_prefix_error() == 0
 
 
+def _runs_case(seed, heads, prefix, groups, order=None):
+    """Requests with several tokens each: groups = [[lengths of the tokens of request 0], ...]."""
+    lens = [n for g in groups for n in g]
+    request = [r for r, g in enumerate(groups) for _ in g]
+    host = np.random.default_rng(seed)
+    c = _case(seed, len(groups), heads, prefix, [max(g) for g in groups])
+    g = _gen(seed + 1)
+    order = list(range(len(lens))) if order is None else host.permutation(len(lens)).tolist()
+    c["lens"], c["request"] = _put(np.array(lens)[order]), _put(np.array(request)[order])
+    c["qn"] = torch.randn((len(lens), heads, DC), generator=g, device="cuda").to(torch.bfloat16)
+    c["qp"] = torch.randn((len(lens), heads, DP), generator=g, device="cuda").to(torch.bfloat16)
+    return c
+
+
+@pytest.mark.parametrize("heads,groups,order", [
+    (16, [[300, 301, 302, 303, 304, 305, 306, 307, 308, 309]], None), (16, [[5, 6, 7], [190, 191, 192, 193, 194], [64, 128]], None),
+    (16, [[128, 0, 129, 64, 63, 1, 65]], None), (32, [[700, 701, 702], [63, 64, 65, 66]], None), (48, [[130, 131], [1], [257, 256]], None),
+    (128, [[100, 101, 102], [0, 0], [64]], None), (16, [[500, 501, 502], [100, 101], [64, 65, 66, 67]], "mixed")])
+def test_prefix_tokens_of_one_request(heads, groups, order):
+    """Tokens of a request side by side share its pages, each up to its own length."""
+    for prefix in (0, 100):
+        c = _runs_case(21, heads, prefix, groups, order)
+        _check_attention(c, _attend(c))
+    assert fi.read_prefix_error() == 0
+
+
+def test_prefix_later_rows_of_the_same_request_are_not_seen():
+    """Rows that a later token of the request sees hold NaN: the earlier tokens' outputs stay as they are."""
+    c = _runs_case(22, 16, 70, [[125, 126, 127, 128, 129, 200]])
+    want = _attend(c)
+    for row in (125, 128, 150):
+        d = {k: v.clone() for k, v in c.items()}
+        d["ckv"][d["table"][0, row // PAGE], row % PAGE] = float("nan")
+        out, lse = _attend(d)
+        sees = d["lens"] > row
+        assert torch.equal(out[~sees], want[0][~sees]) and torch.equal(lse[~sees], want[1][~sees])
+        assert out[sees].isnan().all() and lse[sees].isnan().all()
+
+
+def test_prefix_many_row_blocks():
+    """More row blocks than threads of a CTA, most of them finished by one pair."""
+    lens = np.random.default_rng(5).integers(0, 150, 4200)
+    c = _case(23, 4200, 16, 90, lens)
+    _check_attention(c, _attend(c))
+    c = _case(24, 600, 128, 65, lens[:600] // 4)
+    _check_attention(c, _attend(c))
+
+
 @pytest.mark.parametrize("stale", [float("nan"), float("inf"), -float("inf"), 3e38])
 def test_prefix_rows_behind_a_length_are_not_read(stale):
     c = _case(11, 10, 16, 100, [0, 1, 63, 64, 65, 100, 5, 7, 190, 2], stale=stale)
