@@ -506,25 +506,6 @@ def test_prefix_repeats_bit_for_bit_and_private_workspace():
         _attend(c, workspace=ws[:128])
 
 
-def test_prefix_far_pages():
-    """Cache offsets past 2^31 elements and 2^32 bytes."""
-    pages = 70000
-    ckv = torch.empty((pages, PAGE, DC), dtype=torch.bfloat16, device="cuda")
-    kpe = torch.empty((pages, PAGE, DP), dtype=torch.bfloat16, device="cuda")
-    c = _case(19, 3, 16, 130, [70, 5, 64])
-    n = c["ckv"].shape[0]
-    ckv[pages - n:], kpe[pages - n:] = c["ckv"], c["kpe"]
-    got = fi.shared_prefix_attention(c["qn"], c["qp"], ckv, kpe, c["pages"] + (pages - n), c["prefix"],
-                                     c["table"] + (pages - n), c["lens"], SCALE)
-    _check_attention(c, got)
-    # and the writer: the last row of the cache
-    kv = torch.randn((1, 576), device="cuda").to(torch.bfloat16)
-    w = torch.ones(DC, device="cuda")
-    fi.latent_cache_append(kv, w, _put([3]), _put([pages * PAGE - 1]), fi.rope_frequencies(DP), ckv, kpe)
-    e = _append64(kv, w, _put([3]), fi.rope_frequencies(DP), "interleaved", 1e-6, 1.0)[0]
-    assert ((ckv[-1, -1].double() - e[0]).abs() <= (2 ** -8 + 2e-6) * e[0].abs()).all()
-
-
 def test_wrappers_refuse_on_the_gpu():
     c = _case(20, 2, 16, 10, [3, 4])
     with pytest.raises(RuntimeError, match="CUDA"):
@@ -614,3 +595,25 @@ def test_step_captured_follows_lengths():
         assert torch.equal(out, eager[0]) and torch.equal(lse, eager[1])
         _close_step(_step_oracle(a, lay), out, lse)
     assert fi.read_prefix_error() == 0
+
+
+# ------------------------------------------------- offsets past 32 bits, last:
+# its gigabytes stay in torch's cache, from which the next module's test of free
+# device memory takes its own temporaries (a graph capture empties that cache)
+def test_prefix_far_pages():
+    """Cache offsets past 2^31 elements and 2^32 bytes."""
+    pages = 70000
+    ckv = torch.empty((pages, PAGE, DC), dtype=torch.bfloat16, device="cuda")
+    kpe = torch.empty((pages, PAGE, DP), dtype=torch.bfloat16, device="cuda")
+    c = _case(19, 3, 16, 130, [70, 5, 64])
+    n = c["ckv"].shape[0]
+    ckv[pages - n:], kpe[pages - n:] = c["ckv"], c["kpe"]
+    got = fi.shared_prefix_attention(c["qn"], c["qp"], ckv, kpe, c["pages"] + (pages - n), c["prefix"],
+                                     c["table"] + (pages - n), c["lens"], SCALE)
+    _check_attention(c, got)
+    # and the writer: the last row of the cache
+    kv = torch.randn((1, 576), device="cuda").to(torch.bfloat16)
+    w = torch.ones(DC, device="cuda")
+    fi.latent_cache_append(kv, w, _put([3]), _put([pages * PAGE - 1]), fi.rope_frequencies(DP), ckv, kpe)
+    e = _append64(kv, w, _put([3]), fi.rope_frequencies(DP), "interleaved", 1e-6, 1.0)[0]
+    assert ((ckv[-1, -1].double() - e[0]).abs() <= (2 ** -8 + 2e-6) * e[0].abs()).all()
