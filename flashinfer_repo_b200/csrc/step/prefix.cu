@@ -42,6 +42,8 @@ constexpr int kThreads = 12 * 32;
 constexpr int kSoftmaxThreads = 256;
 constexpr uint32_t kTmemS = 256;               // TMEM columns: O 0-255, scores 256 and 320
 constexpr int kSlotFloats = 2 * kRows * 512 + 4 * kRows;  // partial: O, m, l of 128 rows
+constexpr int kCutTiles = 3;  // what a second row block costs a pair: queries, a refill and a partial, in tiles
+constexpr int kL2Pages = 1300;  // pages of 73728 bytes that stay in the 126 MB of L2 beside the rest
 constexpr float kLazy = 8.f;  // the running maximum follows only a rise of more than 2^8
 
 struct PrefixParams {
@@ -57,8 +59,8 @@ struct PrefixParams {
   float* lse;
   int64_t lse_st, lse_sh;
   int* err;
-  // for the merge grid: tiles before each row block [blocks + 1] and the row
-  // block in which each pair begins [max_pairs]
+  // for the merge grid: tiles before each row block [blocks + 1] and the pairs
+  // that each has of its own, if so; the row block in which each pair begins
   long long* cum;
   int* begins;
   // partials, two a pair: of the stretch's first row block and, where that is
@@ -85,8 +87,8 @@ __device__ __forceinline__ int tokens_of(const PrefixParams& p, int block) {
   const unsigned last = min((unsigned)(block + 1) * kGroups, (unsigned)p.groups) - 1;
   return (int)(last / (unsigned)p.group_per_token) - first_token(p, block) + 1;
 }
-// The tiles are dealt out in stretches of `each`, one more for the first `more`
-// pairs; with fewer tiles than pairs some pairs stay idle.
+// The tiles of all row blocks in one line are dealt out in stretches of `each`,
+// one more for the first `more` pairs; with fewer tiles than pairs some stay idle.
 struct Deal {
   long long each;
   int more, pairs;
@@ -152,9 +154,9 @@ struct PairSmem {
   int valid[4][2];  // rows of the two pages of the last tiles
   uint64_t q_full, q_empty, k_full[3], k_empty[3], v_full[2], v_empty[2], s_full[2], p_full, pv_done;
   uint64_t seg_full[2], seg_empty[2], valid_full[4];
-  long long start;  // tiles before this pair's first row block
+  long long start, u0, u1;  // tiles before this pair's first row block; its stretch
   long long sums[kThreads / 32];
-  int block;
+  int most[kThreads / 32], block;
   uint32_t tmem;
 };
 static_assert(sizeof(PairSmem) <= 232448, "shared memory of a CTA");
@@ -223,30 +225,60 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     if (lane >= o) before += a;
   }
   if (lane == 31) S.sums[warp] = before;
+  const int widest = __reduce_max_sync(0xffffffffu, (int)mine);  // of a row block, where a thread has one
+  if (lane == 0) S.most[warp] = widest;
   __syncthreads();
   before -= mine;
   long long tiles = 0;
+  int most = 0;
 #pragma unroll
   for (int w = 0; w < kThreads / 32; ++w) {
     if (w < warp) before += S.sums[w];
     tiles += S.sums[w];
+    most = max(most, S.most[w]);
   }
+  // Either every row block has `share` pairs of its own, or the line of all
+  // tiles is cut evenly, and then most pairs work on two row blocks: whichever
+  // leaves the last pair less.  Pairs of their own also walk the prefix in step,
+  // so that a page comes from HBM once for all row blocks; where the prefix does
+  // not fit L2 that is worth an eighth (8 tokens of 128 heads behind 131072 rows,
+  // at the clock that the power limit leaves: 251 against 294 us).
   const Deal deal(p, tiles);
-  const long long u0 = pair < deal.pairs ? deal.start(pair) : tiles, u1 = pair < deal.pairs ? deal.start(pair + 1) : tiles;
-  if (blockIdx.x == 0 || (before <= u0 && u0 < before + mine)) {
+  int share = p.max_pairs / p.blocks;
+  long long even = deal.each + (deal.more > 0) + kCutTiles;
+  if (pre_pages > kL2Pages) even += even >> 3;
+  if (share > 0 && (most + share - 1) / share > even) share = 0;
+  if (share > 0) {
+    const int part = pair % share, n = min(share, (int)mine);
+    if ((int)threadIdx.x == pair / share && b0 < b1) {
+      S.block = b0;
+      S.start = before;
+      S.u0 = before + (part < n ? mine * part / n : 0);
+      S.u1 = before + (part < n ? mine * (part + 1) / n : 0);
+    } else if (threadIdx.x == 0 && pair / share >= p.blocks) {
+      S.u0 = S.u1 = 0;
+    }
+  } else if (threadIdx.x == 0) {
+    S.u0 = pair < deal.pairs ? deal.start(pair) : tiles;
+    S.u1 = pair < deal.pairs ? deal.start(pair + 1) : tiles;
+  }
+  const long long at = share > 0 ? 0 : pair < deal.pairs ? deal.start(pair) : tiles;
+  if (blockIdx.x == 0 || (share == 0 && before <= at && at < before + mine)) {
     long long c = before;
     for (int b = b0; b < b1; ++b) {
       const long long n = stretch == 1 ? mine : tiles_of(p, b, pre_pages);
       if (blockIdx.x == 0) p.cum[b] = c;
-      if (c <= u0 && u0 < c + n) {
+      if (share == 0 && c <= at && at < c + n) {
         S.block = b;
         S.start = c;
       }
       c += n;
     }
     if (blockIdx.x == 0 && b1 == p.blocks) p.cum[p.blocks] = tiles;
+    if (blockIdx.x == 0 && threadIdx.x == 0) p.cum[p.blocks + 1] = share;
   }
   __syncthreads();
+  const long long u0 = S.u0, u1 = S.u1;
   if (threadIdx.x == 0 && rank == 0 && u0 < u1) p.begins[pair] = S.block;
 
   if (warp == 11) {
@@ -736,13 +768,22 @@ __global__ void __launch_bounds__(kMergeRows * kMergeColumns)
   const int cut = blockIdx.y + 1;
   int lo = blockIdx.y;
   if (by_cut) lo = p.begins[cut];  // tiles >= blocks >= pairs here: every pair works
-  const Deal deal(p, tiles);
   const long long c0 = p.cum[lo], c1 = p.cum[lo + 1];
-  // a cut on the block's edge is none, and a block is joined once, at its first
-  if (by_cut && (deal.start(cut) == c0 || deal.start(cut - 1) > c0)) return;
-  const int first = deal.pair_of(c0), last = deal.pair_of(c1 - 1);
+  const int share = (int)p.cum[p.blocks + 1];
+  int first, last;
+  bool began_before = false;
+  if (share > 0) {
+    first = lo * share;
+    last = first + (int)min((long long)share, c1 - c0) - 1;
+  } else {
+    const Deal deal(p, tiles);
+    // a cut on the block's edge is none, and a block is joined once, at its first
+    if (by_cut && (deal.start(cut) == c0 || deal.start(cut - 1) > c0)) return;
+    first = deal.pair_of(c0);
+    last = deal.pair_of(c1 - 1);
+    began_before = deal.start(first) < c0;
+  }
   if (first == last) return;  // one pair had it all and wrote the results
-  const bool began_before = deal.start(first) < c0;
   constexpr int kParts = 128 / (kMergeColumns * kQuads);
   const int row = blockIdx.x / kParts * kMergeRows + threadIdx.x % kMergeRows;
   const int quad = blockIdx.x % kParts * (kMergeColumns * kQuads) + threadIdx.x / kMergeRows;
@@ -867,7 +908,7 @@ Layout workspace_layout(int64_t tokens, int64_t heads, int pairs) {
   Layout w;
   w.blocks = (tokens * (heads / 16) + kGroups - 1) / kGroups;
   w.cum = 256;
-  w.begins = w.cum + (w.blocks + 1) * 8;
+  w.begins = w.cum + (w.blocks + 2) * 8;
   w.parts = (w.begins + pairs * 4 + 255) / 256 * 256;
   w.bytes = (size_t)(w.parts + 2 * pairs * (int64_t)kSlotFloats * 4);
   return w;
