@@ -44,6 +44,7 @@ constexpr uint32_t kTmemS = 256;               // TMEM columns: O 0-255, scores 
 constexpr int kSlotFloats = 2 * kRows * 512 + 4 * kRows;  // partial: O, m, l of 128 rows
 constexpr int kCutTiles = 3;  // what a second row block costs a pair: queries, a refill and a partial, in tiles
 constexpr int kL2Pages = 1300;  // pages of 73728 bytes that stay in the 126 MB of L2 beside the rest
+constexpr int kSoloBlocks = 64;  // row blocks that a warp plans alone: 2 a lane
 constexpr float kLazy = 8.f;  // the running maximum follows only a rise of more than 2^8
 
 struct PrefixParams {
@@ -51,6 +52,7 @@ struct PrefixParams {
   int64_t bt_stride;
   int max_prefix, batch, max_own, num_pages;  // max_own: rows that a row of the block table has room for
   int groups, blocks, group_per_token, max_pairs;
+  int share;  // pairs that each row block can have of its own
   int q_boxes;  // query loads of 64 rows
   float scale_log2;  // above zero
   int negate;        // sm_scale is below zero
@@ -172,6 +174,88 @@ __device__ __forceinline__ uint32_t lanes_off(uint32_t sees, int word) {
   return (two & 1 ? 0xffffu : 0u) | (two & 2 ? 0xffff0000u : 0u);
 }
 
+// Where this pair begins and ends, by kWidth threads (a warp or the CTA) that take
+// a stretch of the row blocks each: every CTA adds up all the tiles by itself,
+// which is cheaper than a grid that plans.
+template <int kWidth>
+__device__ __forceinline__ void make_plan(const PrefixParams& p, PairSmem& S, int pair, int idx) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int pre_pages = (int)(((unsigned)prefix_rows(p) + 63) >> 6);
+  const int stretch = (p.blocks + kWidth - 1) / kWidth;
+  const int b0 = min(idx * stretch, p.blocks), b1 = min(b0 + stretch, p.blocks);
+  long long mine = 0;
+  int most = 0;
+  for (int b = b0; b < b1; ++b) {
+    const int n = tiles_of(p, b, pre_pages);
+    mine += n;
+    most = max(most, n);
+  }
+  long long before = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long a = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += a;
+  }
+  most = __reduce_max_sync(0xffffffffu, most);
+  long long tiles = __shfl_sync(0xffffffffu, before, 31);
+  before -= mine;
+  if (kWidth > 32) {
+    if (lane == 0) {
+      S.sums[warp] = tiles;
+      S.most[warp] = most;
+    }
+    __syncthreads();
+    tiles = 0;
+#pragma unroll
+    for (int w = 0; w < kWidth / 32; ++w) {
+      if (w < warp) before += S.sums[w];
+      tiles += S.sums[w];
+      most = max(most, S.most[w]);
+    }
+  }
+  // Either every row block has `share` pairs of its own, or the line of all
+  // tiles is cut evenly, and then most pairs work on two row blocks: whichever
+  // leaves the last pair less.  Pairs of their own also walk the prefix in step,
+  // so that a page comes from HBM once for all row blocks; where the prefix does
+  // not fit L2 that is worth an eighth (8 tokens of 128 heads behind 131072 rows,
+  // at the clock that the power limit leaves: 251 against 294 us).
+  const Deal deal(p, tiles);
+  long long even = deal.each + (deal.more > 0) + kCutTiles;
+  if (pre_pages > kL2Pages) even += even >> 3;
+  const int share = most <= even * p.share ? p.share : 0;
+  const int own_block = share > 0 ? pair / share : -1;
+  const long long at = share > 0 ? -1 : pair < deal.pairs ? deal.start(pair) : tiles;
+  if (idx == 0 && (own_block >= p.blocks || at == tiles)) S.u0 = S.u1 = S.block = 0;  // nothing for this pair
+  if (blockIdx.x == 0 || (b0 <= own_block && own_block < b1) || (before <= at && at < before + mine)) {
+    long long c = before;
+    for (int b = b0; b < b1; ++b) {
+      const int n = stretch == 1 ? (int)mine : tiles_of(p, b, pre_pages);
+      if (blockIdx.x == 0) p.cum[b] = c;
+      if (b == own_block) {
+        const int parts = min(share, n), part = pair - b * share, each = n / parts, more = n - each * parts;
+        S.block = b;
+        S.start = c;
+        S.u0 = c + (part < parts ? each * part + min(part, more) : n);
+        S.u1 = c + (part < parts ? each * (part + 1) + min(part + 1, more) : n);
+      } else if (c <= at && at < c + n) {
+        S.block = b;
+        S.start = c;
+        S.u0 = at;
+        S.u1 = deal.start(pair + 1);
+      }
+      c += n;
+    }
+    if (blockIdx.x == 0 && idx == 0) {
+      p.cum[p.blocks] = tiles;
+      p.cum[p.blocks + 1] = share;
+    }
+  }
+  if (kWidth > 32)
+    __syncthreads();
+  else
+    __syncwarp();
+}
+
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     dsa_prefix_attention_kernel(const __grid_constant__ CUtensorMap map_qn, const __grid_constant__ CUtensorMap map_qp,
                                 const __grid_constant__ CUtensorMap map_ckv3, const __grid_constant__ CUtensorMap map_ckv2,
@@ -211,80 +295,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const uint32_t tmem = S.tmem;
   asm volatile("griddepcontrol.wait;" ::: "memory");  // what ran before is done
 
-  // Every CTA adds up the tiles of all row blocks (each thread a stretch of
-  // them) and finds where its pair begins: cheaper than a grid that plans.
-  const int pre = prefix_rows(p), pre_pages = (int)(((unsigned)pre + 63) >> 6);
-  const int stretch = (p.blocks + kThreads - 1) / kThreads;
-  const int b0 = min((int)threadIdx.x * stretch, p.blocks), b1 = min(b0 + stretch, p.blocks);
-  long long mine = 0;
-  for (int b = b0; b < b1; ++b) mine += tiles_of(p, b, pre_pages);
-  long long before = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long a = __shfl_up_sync(0xffffffffu, before, o);
-    if (lane >= o) before += a;
-  }
-  if (lane == 31) S.sums[warp] = before;
-  const int widest = __reduce_max_sync(0xffffffffu, (int)mine);  // of a row block, where a thread has one
-  if (lane == 0) S.most[warp] = widest;
-  __syncthreads();
-  before -= mine;
-  long long tiles = 0;
-  int most = 0;
-#pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) {
-    if (w < warp) before += S.sums[w];
-    tiles += S.sums[w];
-    most = max(most, S.most[w]);
-  }
-  // Either every row block has `share` pairs of its own, or the line of all
-  // tiles is cut evenly, and then most pairs work on two row blocks: whichever
-  // leaves the last pair less.  Pairs of their own also walk the prefix in step,
-  // so that a page comes from HBM once for all row blocks; where the prefix does
-  // not fit L2 that is worth an eighth (8 tokens of 128 heads behind 131072 rows,
-  // at the clock that the power limit leaves: 251 against 294 us).
-  const Deal deal(p, tiles);
-  int share = p.max_pairs / p.blocks;
-  long long even = deal.each + (deal.more > 0) + kCutTiles;
-  if (pre_pages > kL2Pages) even += even >> 3;
-  if (share > 0 && (most + share - 1) / share > even) share = 0;
-  if (share > 0) {
-    const int part = pair % share, n = min(share, (int)mine);
-    if ((int)threadIdx.x == pair / share && b0 < b1) {
-      S.block = b0;
-      S.start = before;
-      S.u0 = before + (part < n ? mine * part / n : 0);
-      S.u1 = before + (part < n ? mine * (part + 1) / n : 0);
-    } else if (threadIdx.x == 0 && pair / share >= p.blocks) {
-      S.u0 = S.u1 = 0;
-    }
-  } else if (threadIdx.x == 0) {
-    S.u0 = pair < deal.pairs ? deal.start(pair) : tiles;
-    S.u1 = pair < deal.pairs ? deal.start(pair + 1) : tiles;
-  }
-  const long long at = share > 0 ? 0 : pair < deal.pairs ? deal.start(pair) : tiles;
-  if (blockIdx.x == 0 || (share == 0 && before <= at && at < before + mine)) {
-    long long c = before;
-    for (int b = b0; b < b1; ++b) {
-      const long long n = stretch == 1 ? mine : tiles_of(p, b, pre_pages);
-      if (blockIdx.x == 0) p.cum[b] = c;
-      if (share == 0 && c <= at && at < c + n) {
-        S.block = b;
-        S.start = c;
-      }
-      c += n;
-    }
-    if (blockIdx.x == 0 && b1 == p.blocks) p.cum[p.blocks] = tiles;
-    if (blockIdx.x == 0 && threadIdx.x == 0) p.cum[p.blocks + 1] = share;
-  }
-  __syncthreads();
-  const long long u0 = S.u0, u1 = S.u1;
-  if (threadIdx.x == 0 && rank == 0 && u0 < u1) p.begins[pair] = S.block;
+  // few row blocks: the warp that cuts segments plans alone, no other waits
+  const bool alone = p.blocks <= kSoloBlocks;
+  if (!alone) make_plan<kThreads>(p, S, pair, threadIdx.x);
 
   if (warp == 11) {
     // ------------------------------------------------------------- segments
+    if (alone) make_plan<32>(p, S, pair, lane);
+    const int pre = prefix_rows(p), pre_pages = (int)(((unsigned)pre + 63) >> 6);
+    const long long u1 = S.u1;
     int block = S.block;
-    long long u = u0, c0 = S.start;
+    long long u = S.u0, c0 = S.start;
+    if (rank == 0 && lane == 0 && u < u1) p.begins[pair] = block;
     for (int n = 0;; ++n) {
       const int s = n & 1;
       if (!mbar_wait(&S.seg_empty[s], ((n >> 1) & 1) ^ 1)) {
@@ -1024,6 +1046,7 @@ extern "C" int dsa_shared_prefix_attention(
   p.groups = (int)(num_tokens * gpt);
   p.blocks = (int)w.blocks;
   p.max_pairs = pairs;
+  p.share = pairs / p.blocks;
   p.q_boxes = q_boxes;
   // scores are scaled after the maximum is taken: a scale below zero turns them
   // over first, and zero becomes a scale that makes every score nothing
