@@ -110,6 +110,9 @@ def call(fn_name: str, *args):
 
 
 _bound = {}
+# the raw getters: torch.cuda.current_stream builds an object, 1.5 us a call
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else None
+_current_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
 
 
 def call_on(index: int, fn_name: str, *args):
@@ -118,26 +121,33 @@ def call_on(index: int, fn_name: str, *args):
     f = _bound.get(fn_name)
     if f is None:
         f = _bound[fn_name] = getattr(load(), fn_name)
-    # the raw getters: torch.cuda.current_stream builds an object, 1.5 us a call
-    if torch._C._cuda_getDevice() == index:
-        rc = f(*args, torch._C._cuda_getCurrentRawStream(index))
+    if _current_device() == index:
+        rc = f(*args, _current_stream(index))
     else:
         with torch.cuda.device(index):
-            rc = f(*args, torch._C._cuda_getCurrentRawStream(index))
+            rc = f(*args, _current_stream(index))
     if rc != 0:
         check(fn_name, rc)
 
 
-def same_device(**tensors) -> int:
-    """Index of the one CUDA device that every tensor (None is skipped) is on;
+def same_device(first, *others) -> int:
+    """Index of the one CUDA device that all tensors (None is skipped) are on;
     RuntimeError if they are on several or on the CPU."""
-    index = -1
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        at = t.get_device()
-        if at != index or at < 0:
-            if index >= 0 or at < 0:
-                raise RuntimeError(f"{name} must be a CUDA tensor on the other tensors' device (no CPU path), got {t.device}")
-            index = at
+    index = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != index:
+            index = -1
+            break
+    if index < 0:
+        where = [str(t.device) for t in (first, *others) if t is not None]
+        raise RuntimeError(f"all tensors must be on one CUDA device (no CPU path), got {where}")
     return index
+
+
+def int32(t, name: str):
+    """Contiguous int32 copy of an id or length tensor (itself if it is one);
+    64-bit values past 32 bits are cut to the range's ends, not wrapped around."""
+    if t.dtype == torch.int32:
+        return t if t.is_contiguous() else t.contiguous()
+    assert t.dtype == torch.int64, f"{name} must be int32 or int64"
+    return t.clamp(-2 ** 31, 2 ** 31 - 1).to(torch.int32).contiguous()

@@ -129,16 +129,13 @@ __global__ void __launch_bounds__(kLayThreads) dsa_step_layout_kernel(const Layo
       const long long col = pos >> 6, have = ((long long)seq[b] + 63) >> 6;
       int32_t page = -1;
       if (col < p.max_pages) {
-        if (col < have) {
-          page = p.table[(b0 + b) * p.bt_stride + col];
-          if (page < 0) bits |= kErrBadIndex;
-        } else {
-          const long long src = pages_base + page0[b] + (col - have);
-          if (src < p.num_free) page = p.free_pages[src];
-        }
+        const long long src = pages_base + page0[b] + (col - have);
+        const bool have_it = col < have || src < p.num_free;
+        if (have_it) page = col < have ? p.table[(b0 + b) * p.bt_stride + col] : p.free_pages[src];
+        // a slot past 2^31 rows has no 32-bit id: no cache of this library is that long
+        if (have_it && (page < 0 || page >= (1 << 25))) bits |= kErrBadIndex;
       }
       const long long out = rows_base + i;
-      // a slot past 2^31 rows has no 32-bit id: no cache of this library is that long
       const bool ok = page >= 0 && page < (1 << 25);
       p.slots[out] = ok ? page * 64 + (int)(pos & 63) : -1;
       p.positions[out] = (int32_t)min(prefix + pos, (long long)INT32_MAX);

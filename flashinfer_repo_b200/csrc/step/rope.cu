@@ -209,8 +209,8 @@ extern "C" int dsa_apply_rope(const void* x, int64_t x_stride_token, int64_t x_s
     return report_error(DSA_ERR_UNSUPPORTED, "rotated width must be even, 2 to 512");
   if (rot_offset + rot_dim > head_dim)
     return report_error(DSA_ERR_INVALID_ARG, "rotated slice reaches past the head");
-  if (num_heads > 65535 || head_dim > 65535)
-    return report_error(DSA_ERR_UNSUPPORTED, "at most 65535 heads of at most 65535 values");
+  if (num_heads > 65535 || head_dim > 65535 || num_heads * head_dim > (1 << 28))
+    return report_error(DSA_ERR_UNSUPPORTED, "at most 65535 heads of at most 65535 values, and 2^28 values a token");
   if (layout != DSA_ROPE_INTERLEAVED && layout != DSA_ROPE_HALF)
     return report_error(DSA_ERR_INVALID_ARG, "unknown rotary layout");
   if (dtype != DSA_BF16 && dtype != DSA_FP16 && dtype != DSA_FP32)

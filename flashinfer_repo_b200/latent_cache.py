@@ -35,18 +35,16 @@ def latent_cache_append(kv, norm_weight, positions, slots, inv_freq, ckv_cache, 
     assert ckv_cache.dtype == torch.bfloat16 and kpe_cache.dtype == torch.bfloat16, "the caches are bf16"
     assert ckv_cache.shape == (num_pages, PAGE_SIZE, HEAD_DIM_CKV)
     assert kpe_cache.shape == (num_pages, PAGE_SIZE, HEAD_DIM_KPE)
-    assert slots.shape == (tokens,) and slots.dtype in (torch.int32, torch.int64), "slots must be [tokens] int32 or int64"
+    assert slots.shape == (tokens,), "slots must be [tokens]"
     assert inv_freq.shape == (HEAD_DIM_KPE // 2,), "inv_freq must have 32 values"
-    index = _lib.same_device(kv=kv, norm_weight=norm_weight, positions=positions, slots=slots, inv_freq=inv_freq,
-                             ckv_cache=ckv_cache, kpe_cache=kpe_cache, device_error=device_error)
+    index = _lib.same_device(kv, norm_weight, positions, slots, inv_freq, ckv_cache, kpe_cache, device_error)
     positions, inv_freq = _check_rotation(positions, inv_freq, tokens, layout)
     if device_error is not None:
         assert device_error.dtype == torch.int32 and device_error.numel() >= 1, "device_error must be int32"
     if kv.stride(1) != 1:
         kv = kv.contiguous()
     norm_weight = norm_weight.contiguous()
-    if slots.dtype != torch.int32 or not slots.is_contiguous():
-        slots = slots.to(torch.int32).contiguous()
+    slots = _lib.int32(slots, "slots")
     c_page, c_row, c_last = ckv_cache.stride()
     e_page, e_row, e_last = kpe_cache.stride()
     assert c_last == 1 and e_last == 1, "cache rows must be contiguous"

@@ -28,11 +28,6 @@ class StepLayout(NamedTuple):
     pages_used: torch.Tensor     # [1]: free pages taken
 
 
-def _lens(t: torch.Tensor, name: str) -> torch.Tensor:
-    assert t.dim() == 1 and t.dtype in (torch.int32, torch.int64), f"{name} must be [requests] int32 or int64"
-    return t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
-
-
 def step_layout(seq_lens, query_lens, block_table, free_pages, num_tokens, *, prefix_len=None, out=None,
                 device_error=None) -> StepLayout:
     """Lay out a step: pages for the new rows, and where each new row goes.
@@ -48,15 +43,16 @@ def step_layout(seq_lens, query_lens, block_table, free_pages, num_tokens, *, pr
     of pages, table columns or rows; 1: a negative entry of an older page).
     Calling it again with the same lengths and free pages gives the same result.
     """
-    seq_lens, query_lens = _lens(seq_lens, "seq_lens"), _lens(query_lens, "query_lens")
-    free_pages = _lens(free_pages, "free_pages")
+    seq_lens, query_lens = _lib.int32(seq_lens, "seq_lens"), _lib.int32(query_lens, "query_lens")
+    free_pages = _lib.int32(free_pages, "free_pages")
+    assert seq_lens.dim() == 1 and query_lens.dim() == 1 and free_pages.dim() == 1
     num_tokens = int(num_tokens)
     batch, width = block_table.shape
     assert seq_lens.shape[0] == batch and query_lens.shape[0] == batch and num_tokens >= 0
     assert block_table.dtype == torch.int32 and (width <= 1 or block_table.stride(1) == 1), \
         "block_table must be int32 with contiguous rows"
-    index = _lib.same_device(block_table=block_table, seq_lens=seq_lens, query_lens=query_lens, free_pages=free_pages,
-                             prefix_len=prefix_len, device_error=device_error)
+    assert prefix_len is None or isinstance(prefix_len, torch.Tensor), "prefix_len must be one int32 on the GPU"
+    index = _lib.same_device(block_table, seq_lens, query_lens, free_pages, prefix_len, device_error)
     if prefix_len is not None:
         assert prefix_len.dtype == torch.int32 and prefix_len.numel() == 1, "prefix_len must be one int32"
     if device_error is not None:
@@ -67,7 +63,7 @@ def step_layout(seq_lens, query_lens, block_table, free_pages, num_tokens, *, pr
         at = buf.data_ptr()
         outs = tuple(at + 4 * num_tokens * i for i in range(5))
     else:
-        assert _lib.same_device(**out._asdict()) == index, "out: on the inputs' device"
+        assert _lib.same_device(*out) == index, "out: on the inputs' device"
         for t, n in zip(out, (num_tokens,) * 4 + (1,)):
             assert t.dtype == torch.int32 and t.numel() == n and t.is_contiguous(), "out: int32, contiguous"
         outs = tuple(t.data_ptr() for t in out)

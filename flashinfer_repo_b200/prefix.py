@@ -9,6 +9,7 @@ document).  The reference has no counterpart.
 from __future__ import annotations
 
 import ctypes
+import threading
 
 import torch
 
@@ -16,6 +17,7 @@ from . import _lib
 from .kernel import HEAD_DIM_CKV, HEAD_DIM_KPE, NUM_HEADS, PAGE_SIZE
 
 _workspaces: dict[int, list] = {}  # per device: every buffer handed out, the newest last
+_lock = threading.Lock()
 _size_cache: dict[tuple, int] = {}
 
 
@@ -40,17 +42,18 @@ def _index(device) -> int:
 
 
 def _workspace(index: int, nbytes: int) -> torch.Tensor:
-    """The device's shared workspace.  A larger call gets a new buffer, half as
-    large again at least; older ones are kept, since a captured graph may hold
-    their address."""
-    kept = _workspaces.setdefault(index, [])
+    """The device's shared workspace.  Few calls outgrow it (its size hardly
+    depends on the shape); they get a new one, and the old one is kept, since a
+    captured graph may hold its address."""
+    kept = _workspaces.get(index)
     if not kept or kept[-1].numel() < nbytes:
-        nbytes = max(nbytes, kept[-1].numel() * 3 // 2 // 256 * 256 if kept else 0)
-        with torch.cuda.device(index):
-            if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("the workspace must grow during stream capture: make one call of this size before "
-                                   "the capture, or pass workspace=")
-            kept.append(torch.zeros(nbytes, dtype=torch.uint8, device=f"cuda:{index}"))
+        with _lock, torch.cuda.device(index):
+            kept = _workspaces.setdefault(index, [])
+            if not kept or kept[-1].numel() < nbytes:
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("the workspace must grow during stream capture: make one call of this size "
+                                       "before the capture, or pass workspace=")
+                kept.append(torch.zeros(nbytes + (4 << 20), dtype=torch.uint8, device=f"cuda:{index}"))
     return kept[-1]
 
 
@@ -81,16 +84,14 @@ def shared_prefix_attention(q_nope, q_pe, ckv_cache, kpe_cache, prefix_pages, pr
     assert ckv_cache.shape == (num_pages, PAGE_SIZE, HEAD_DIM_CKV)
     assert kpe_cache.shape == (num_pages, PAGE_SIZE, HEAD_DIM_KPE)
     length = prefix_len if isinstance(prefix_len, torch.Tensor) else None
-    index = _lib.same_device(q_nope=q_nope, q_pe=q_pe, ckv_cache=ckv_cache, kpe_cache=kpe_cache,
-                             prefix_pages=prefix_pages, prefix_len=length, block_table=block_table,
-                             token_lens=token_lens, token_request=token_request, output=output, lse=lse,
-                             workspace=workspace)
+    index = _lib.same_device(q_nope, q_pe, ckv_cache, kpe_cache, prefix_pages, length, block_table, token_lens,
+                             token_request, output, lse, workspace)
     bf16 = torch.bfloat16
     assert q_nope.dtype == bf16 and q_pe.dtype == bf16 and ckv_cache.dtype == bf16 and kpe_cache.dtype == bf16, \
         "queries and caches must be bfloat16"
     requests, width = block_table.shape
     assert token_lens.shape == (tokens,), "token_lens must be [tokens]"
-    prefix_pages, token_lens = _int32(prefix_pages, "prefix_pages"), _int32(token_lens, "token_lens")
+    prefix_pages, token_lens = _lib.int32(prefix_pages, "prefix_pages"), _lib.int32(token_lens, "token_lens")
     if length is not None:
         assert length.numel() == 1 and length.dtype == torch.int32, "prefix_len must be an int or one int32"
         bound = prefix_pages.shape[0] * PAGE_SIZE
@@ -99,7 +100,7 @@ def shared_prefix_attention(q_nope, q_pe, ckv_cache, kpe_cache, prefix_pages, pr
         assert 0 <= bound <= prefix_pages.shape[0] * PAGE_SIZE, "prefix_len does not fit prefix_pages"
     if token_request is not None:
         assert token_request.shape == (tokens,), "token_request must be [tokens]"
-        token_request = _int32(token_request, "token_request")
+        token_request = _lib.int32(token_request, "token_request")
     else:
         assert requests >= tokens, "without token_request the block table needs a row for every token"
     if output is None:
@@ -116,7 +117,7 @@ def shared_prefix_attention(q_nope, q_pe, ckv_cache, kpe_cache, prefix_pages, pr
         return output, lse
     assert num_pages > 0, "the cache has no pages"
     if block_table.dtype != torch.int32 or (width > 1 and block_table.stride(1) != 1):
-        block_table = _int32(block_table, "block_table")
+        block_table = _lib.int32(block_table, "block_table")
     q_nope, qn_token, qn_head = _tiled(q_nope)
     q_pe, qp_token, qp_head = _tiled(q_pe)
     rows_c, c_page, c_row = _tiled(ckv_cache)
@@ -145,13 +146,6 @@ def _tiled(t: torch.Tensor):
         return t, outer, inner
     t = t.clone(memory_format=torch.contiguous_format)
     return t, t.stride(0), t.stride(1)
-
-
-def _int32(t: torch.Tensor, name: str) -> torch.Tensor:
-    if t.dtype == torch.int32 and t.is_contiguous():
-        return t
-    assert t.dtype in (torch.int32, torch.int64), f"{name} must be int32 or int64"
-    return t.to(torch.int32).contiguous()
 
 
 def read_prefix_error(device=None, clear=True) -> int:

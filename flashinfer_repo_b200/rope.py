@@ -77,7 +77,7 @@ def apply_rope(x, positions, inv_freq, *, layout="interleaved", offset=0, invers
     assert len(shape) in (2, 3), "x must be [tokens, heads, dim] or [tokens, dim]"
     dtype = DTYPES.get(x.dtype)
     assert dtype is not None, f"x must be bf16, fp16 or fp32, got {x.dtype}"
-    index = _lib.same_device(x=x, positions=positions, inv_freq=inv_freq, out=out)
+    index = _lib.same_device(x, positions, inv_freq, out)
     positions, inv_freq = _check_rotation(positions, inv_freq, shape[0], layout)
     rot = 2 * inv_freq.shape[0]
     assert 0 <= offset and offset + rot <= shape[-1], "the rotated slice reaches past the head"
@@ -88,6 +88,7 @@ def apply_rope(x, positions, inv_freq, *, layout="interleaved", offset=0, invers
         out = x.new_empty(shape)
     else:
         assert out.shape == shape and out.dtype == x.dtype and out.stride(-1) == 1
+        assert all(st > 0 for st, n in zip(out.stride(), shape) if n > 1), "out is an expanded tensor"
         assert out.data_ptr() != x.data_ptr() or out.stride() == x.stride(), "out shares x's memory with other strides"
     if len(shape) == 3:
         heads, x_head, o_head = shape[1], x.stride(1), out.stride(1)

@@ -335,8 +335,8 @@ int dsa_index_cache_append(const void* keys_bf16, int64_t num_tokens, const int3
  * *pages_used receives how many free pages were taken.  Running the same step
  * again writes the same values.  Where free pages, table columns or output rows
  * run out, the rows concerned get slot -1 (table entry -1) or are dropped and
- * DSA_DEVERR_CAPACITY is set; a negative entry of an older page gives slot -1
- * and DSA_DEVERR_BAD_INDEX.  device_error may be NULL.  No counterpart in the
+ * DSA_DEVERR_CAPACITY is set; a page id below 0 or past 2^25 gives slot -1 and
+ * DSA_DEVERR_BAD_INDEX.  device_error may be NULL.  No counterpart in the
  * reference, whose caller builds these on the host.
  */
 int dsa_step_layout(const int32_t* seq_lens, const int32_t* query_lens, int64_t batch,
@@ -354,7 +354,7 @@ int dsa_step_layout(const int32_t* seq_lens, const int32_t* query_lens, int64_t 
  * inverse != 0 turns back, which with the same scale is also the gradient.
  * Strides are in elements, the last dimension is contiguous; out may be x (then
  * only the slice is written) but must not overlap it in another way.  rot_dim is
- * even, at most 512.  positions are int32 or int64.  No counterpart in the
+ * even, at most 512; a token has at most 2^28 values.  positions are int32 or int64.  No counterpart in the
  * reference, which takes rotated queries and keys.
  */
 int dsa_apply_rope(const void* x, int64_t x_stride_token, int64_t x_stride_head, void* out,

@@ -250,6 +250,20 @@ def test_append(tokens, layout, dtype):
         assert err.item() == 0
 
 
+def test_ids_past_32_bits_are_flagged_not_wrapped():
+    kv = torch.ones((2, 576), device="cuda", dtype=torch.bfloat16)
+    ckv = torch.zeros((2, PAGE, DC), device="cuda", dtype=torch.bfloat16)
+    kpe = torch.zeros((2, PAGE, DP), device="cuda", dtype=torch.bfloat16)
+    err = torch.zeros(1, dtype=I32, device="cuda")
+    fi.latent_cache_append(kv, torch.ones(DC, device="cuda"), _put([0, 0], torch.int64),
+                           torch.tensor([1 << 32, -(1 << 40)], device="cuda"), fi.rope_frequencies(DP), ckv, kpe,
+                           device_error=err)
+    assert err.item() == 1 and ckv.count_nonzero().item() == 0
+    table = torch.zeros((1, 2), dtype=I32, device="cuda")
+    lay = fi.step_layout(_put([0]), _put([1]), table, torch.tensor([1 << 33], device="cuda"), 1, device_error=err.zero_())
+    assert err.item() == 1 and lay.slots.tolist() == [-1]
+
+
 def test_append_bad_slots_and_int64():
     kv = torch.ones((3, 576), device="cuda", dtype=torch.bfloat16)
     ckv = torch.zeros((2, PAGE, DC), device="cuda", dtype=torch.bfloat16)
@@ -519,6 +533,18 @@ def test_wrappers_refuse_on_the_gpu():
     x = torch.zeros((2, 4, 64), device="cuda")
     with pytest.raises(AssertionError):
         fi.apply_rope(x, _put([1, 2]), fi.rope_frequencies(64), out=x.as_strided((2, 4, 64), (64, 128, 1)))
+    with pytest.raises(AssertionError):
+        fi.apply_rope(x, _put([1, 2]), fi.rope_frequencies(64), out=torch.zeros((2, 1, 64), device="cuda").expand(2, 4, 64))
+    with pytest.raises(AssertionError):
+        fi.step_layout(_put([1]), _put([1]), torch.zeros((1, 2), dtype=I32, device="cuda"), _put([1]), 1, prefix_len=3)
+    with pytest.raises(RuntimeError, match="capture"):
+        graph = torch.cuda.CUDAGraph()
+        big = torch.zeros((1 << 15, 16, 512), dtype=torch.bfloat16, device="cuda")
+        fi.prefix._workspaces.pop(0, None)  # as in a process whose first call is the captured one
+        with torch.cuda.graph(graph):
+            fi.shared_prefix_attention(big, big[..., :64], c["ckv"], c["kpe"], c["pages"], 10, c["table"],
+                                       torch.zeros(1 << 15, dtype=I32, device="cuda"), SCALE,
+                                       token_request=torch.zeros(1 << 15, dtype=I32, device="cuda"))
 
 
 # ------------------------------------------------------------ all together
