@@ -105,14 +105,18 @@ def shared_prefix_attention(q_nope, q_pe, ckv_cache, kpe_cache, prefix_pages, pr
         assert requests >= tokens, "without token_request the block table needs a row for every token"
     if output is None:
         output = q_nope.new_empty((tokens, heads, HEAD_DIM_CKV))
+        out_token, out_head = heads * HEAD_DIM_CKV, HEAD_DIM_CKV
     else:
         assert output.shape == (tokens, heads, HEAD_DIM_CKV) and output.dtype == bf16
-        assert output.stride(-1) == 1 and output.stride(0) % 8 == 0 and output.stride(1) % 8 == 0 \
-            and output.data_ptr() % 16 == 0, "output rows must be contiguous and 16-byte aligned"
+        out_token, out_head, last = output.stride()
+        assert last == 1 and out_token % 8 == 0 and out_head % 8 == 0 and output.data_ptr() % 16 == 0, \
+            "output rows must be contiguous and 16-byte aligned"
     if lse is None:
         lse = q_nope.new_empty((tokens, heads), dtype=torch.float32)
+        lse_token, lse_head = heads, 1
     else:
         assert lse.shape == (tokens, heads) and lse.dtype == torch.float32
+        lse_token, lse_head = lse.stride()
     if tokens == 0:
         return output, lse
     assert num_pages > 0, "the cache has no pages"
@@ -132,14 +136,17 @@ def shared_prefix_attention(q_nope, q_pe, ckv_cache, kpe_cache, prefix_pages, pr
                  prefix_pages.data_ptr(), bound, length.data_ptr() if length is not None else None,
                  block_table.data_ptr(), block_table.stride(0), requests, width,
                  token_request.data_ptr() if token_request is not None else None, token_lens.data_ptr(), tokens,
-                 heads, num_pages, sm_scale, output.data_ptr(), output.stride(0), output.stride(1),
-                 lse.data_ptr(), lse.stride(0), lse.stride(1), workspace.data_ptr(), workspace.numel())
+                 heads, num_pages, sm_scale, output.data_ptr(), out_token, out_head, lse.data_ptr(), lse_token,
+                 lse_head, workspace.data_ptr(), workspace.numel())
     return output, lse
 
 
 def _tiled(t: torch.Tensor):
     """(t, outer, inner stride) of t [A, B, width] if the TMA can read its rows
     where they are, else of a contiguous copy."""
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+        _, rows, width = t.shape
+        return t, rows * width, width
     outer, inner, last = t.stride()
     if last == 1 and inner % 8 == 0 and inner >= t.shape[2] and t.data_ptr() % 16 == 0 and (
             t.shape[0] == 1 or (outer >= inner and outer % 8 == 0)):
