@@ -6,6 +6,10 @@
 
 namespace dsa {
 
+// The two halves of cluster_sync_all.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+
 // One lane of a converged warp (the same one every time).
 __device__ __forceinline__ bool elect_one() {
   uint32_t p;

@@ -292,18 +292,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   if (warp == 9) tmem_alloc_pair(&S.tmem, 512);
   tc_fence_before();
   __syncthreads();
-  cluster_sync_all();  // both CTAs' barriers and TMEM are there
+  cluster_arrive();
+  // few row blocks: the warp that cuts segments plans alone, while the pair meets
+  const bool alone = p.blocks <= kSoloBlocks;
+  if (alone && warp == 11) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // what ran before is done
+    make_plan<32>(p, S, pair, lane);
+  }
+  cluster_wait();  // both CTAs' barriers and TMEM are there
   tc_fence_after();
   const uint32_t tmem = S.tmem;
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // what ran before is done
-
-  // few row blocks: the warp that cuts segments plans alone, no other waits
-  const bool alone = p.blocks <= kSoloBlocks;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (!alone) make_plan<kThreads>(p, S, pair, threadIdx.x);
 
   if (warp == 11) {
     // ------------------------------------------------------------- segments
-    if (alone) make_plan<32>(p, S, pair, lane);
     const int pre = prefix_rows(p), pre_pages = (int)(((unsigned)pre + 63) >> 6);
     const long long u1 = S.u1;
     int block = S.block;
@@ -421,7 +424,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       };
       int next_id, next_rows, id = 0, rows = 0;
       look_up(0, &next_id, &next_rows);
-      if (keys) {
+      // queries: of the first segment by the warp that waits longest for its own
+      // loads, later by the one that sees the queries' last use first
+      if (keys == (n > 0)) {
         if (!mbar_wait(&S.q_empty, (n & 1) ^ 1)) {
           ok = false;
           break;
