@@ -78,7 +78,7 @@ def test_layout_small(seq, q, rows, prefix):
     assert err == 0 and bits == 0
 
 
-@pytest.mark.parametrize("batch", [1, 31, 2047, 2048, 2049, 5000])
+@pytest.mark.parametrize("batch", [1, 31, 511, 512, 513, 2048, 5000])
 def test_layout_many_requests(batch):
     """Batches around the chunk of the scan, decode rows with some chunks and idle requests."""
     rng = np.random.default_rng(batch)
