@@ -30,13 +30,16 @@ struct AppendParams {
   int* err;
 };
 
-// 8 values from `from` on as they are wanted in the sum: 32 bits.
-template <typename T, bool kVec>
+// 8 values from `from` on as they are wanted in the sum: 32 bits.  kOnce: nobody
+// reads them again (first to leave L2: 16384 rows 10.1 -> 9.1 us from cold).
+template <typename T, bool kVec, bool kOnce>
 __device__ __forceinline__ void load8(const T* from, float* v) {
   if (kVec) {
 #pragma unroll
     for (int k = 0; k < 8 / Vec<T>::kN; ++k) {
-      const Vec<T> x = reinterpret_cast<const Vec<T>*>(from)[k];
+      const uint4* at = reinterpret_cast<const uint4*>(from) + k;
+      const uint4 raw = kOnce ? __ldcs(at) : *at;
+      const Vec<T>& x = reinterpret_cast<const Vec<T>&>(raw);
 #pragma unroll
       for (int i = 0; i < Vec<T>::kN; ++i) v[k * Vec<T>::kN + i] = to_f32(x.v[i]);
     }
@@ -46,8 +49,12 @@ __device__ __forceinline__ void load8(const T* from, float* v) {
   }
 }
 
+// 4 rows a CTA: with 8 a decode step took 1.97 instead of 1.78 us, 16384 rows 9.1
+// instead of 8.2.
+constexpr int kAppendThreads = 128;
+
 template <typename T, typename W, bool kVec>
-__global__ void __launch_bounds__(256) dsa_latent_append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(kAppendThreads) dsa_latent_append_kernel(const AppendParams p) {
   const int64_t row = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
   const int lane = threadIdx.x & 31;
   if (row >= p.rows) return;
@@ -57,12 +64,12 @@ __global__ void __launch_bounds__(256) dsa_latent_append_kernel(const AppendPara
   const W* w = static_cast<const W*>(p.w);
   const int ia = p.half_layout ? lane : 2 * lane, ib = p.half_layout ? lane + 32 : 2 * lane + 1;
   float v[2][8], g[2][8];
-  load8<T, kVec>(x + lane * 8, v[0]);
-  load8<T, kVec>(x + 256 + lane * 8, v[1]);
+  load8<T, kVec, true>(x + lane * 8, v[0]);
+  load8<T, kVec, true>(x + 256 + lane * 8, v[1]);
   const float a = to_f32(x[kLatent + ia]), b = to_f32(x[kLatent + ib]);
   const int64_t position = load_position(p.positions, p.pos64, row);
-  load8<W, kVec>(w + lane * 8, g[0]);
-  load8<W, kVec>(w + 256 + lane * 8, g[1]);
+  load8<W, kVec, false>(w + lane * 8, g[0]);
+  load8<W, kVec, false>(w + 256 + lane * 8, g[1]);
   const double freq = p.inv_freq[lane];
   if (slot < 0) {  // a padded row; anything below -1 is a wrong id
     if (slot < -1 && lane == 0) set_error(p.err, kErrBadIndex);
@@ -101,14 +108,14 @@ __global__ void __launch_bounds__(256) dsa_latent_append_kernel(const AppendPara
 
 template <typename T, typename W>
 void launch(const AppendParams& p, cudaStream_t stream) {
-  const unsigned grid = (unsigned)((p.rows * 32 + 255) / 256);
+  const unsigned grid = (unsigned)((p.rows * 32 + kAppendThreads - 1) / kAppendThreads);
   // 16-byte accesses where every row, the weights and the latent cache allow them
   bool vec = p.kv_st % Vec<T>::kN == 0 && p.ckv_sp % 8 == 0 && p.ckv_sr % 8 == 0;
   for (const void* q : {p.kv, p.w, (const void*)p.ckv}) vec = vec && (reinterpret_cast<uintptr_t>(q) & 15) == 0;
   if (vec)
-    dsa_latent_append_kernel<T, W, true><<<grid, 256, 0, stream>>>(p);
+    dsa_latent_append_kernel<T, W, true><<<grid, kAppendThreads, 0, stream>>>(p);
   else
-    dsa_latent_append_kernel<T, W, false><<<grid, 256, 0, stream>>>(p);
+    dsa_latent_append_kernel<T, W, false><<<grid, kAppendThreads, 0, stream>>>(p);
 }
 template <typename T>
 void launch(const AppendParams& p, int w_dtype, cudaStream_t stream) {

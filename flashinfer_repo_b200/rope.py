@@ -81,20 +81,21 @@ def apply_rope(x, positions, inv_freq, *, layout="interleaved", offset=0, invers
     positions, inv_freq = _check_rotation(positions, inv_freq, shape[0], layout)
     rot = 2 * inv_freq.shape[0]
     assert 0 <= offset and offset + rot <= shape[-1], "the rotated slice reaches past the head"
-    if x.stride(-1) != 1:
+    x_at = x.stride()
+    if x_at[-1] != 1:
         assert out is None or out.data_ptr() != x.data_ptr(), "in place needs contiguous heads"
         x = x.contiguous()
+        x_at = x.stride()
     if out is None:
         out = x.new_empty(shape)
+        o_at = out.stride()
     else:
-        assert out.shape == shape and out.dtype == x.dtype and out.stride(-1) == 1
-        assert all(st > 0 for st, n in zip(out.stride(), shape) if n > 1), "out is an expanded tensor"
-        assert out.data_ptr() != x.data_ptr() or out.stride() == x.stride(), "out shares x's memory with other strides"
-    if len(shape) == 3:
-        heads, x_head, o_head = shape[1], x.stride(1), out.stride(1)
-    else:
-        heads, x_head, o_head = 1, 0, 0
-    _lib.call_on(index, "dsa_apply_rope", x.data_ptr(), x.stride(0), x_head, out.data_ptr(), out.stride(0), o_head,
-                 dtype, shape[0], heads, shape[-1], offset, rot, positions.data_ptr(),
-                 positions.dtype == torch.int64, inv_freq.data_ptr(), LAYOUTS[layout], bool(inverse), scale)
+        o_at = out.stride()
+        assert out.shape == shape and out.dtype == x.dtype and o_at[-1] == 1
+        assert all(st > 0 for st, n in zip(o_at, shape) if n > 1), "out is an expanded tensor"
+        assert out.data_ptr() != x.data_ptr() or o_at == x_at, "out shares x's memory with other strides"
+    heads, x_head, o_head = (shape[1], x_at[1], o_at[1]) if len(shape) == 3 else (1, 0, 0)
+    _lib.call_on(index, "dsa_apply_rope", x.data_ptr(), x_at[0], x_head, out.data_ptr(), o_at[0], o_head, dtype,
+                 shape[0], heads, shape[-1], offset, rot, positions.data_ptr(), positions.dtype == torch.int64,
+                 inv_freq.data_ptr(), LAYOUTS[layout], bool(inverse), scale)
     return out
