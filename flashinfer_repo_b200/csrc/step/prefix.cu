@@ -789,13 +789,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 // ----------------------------------------------------------------- merge
 // Rows whose block several pairs share: with partials (O_k, m_k, l_k),
 //   o = sum_k 2^(m_k - M) O_k / sum_k 2^(m_k - M) l_k.
-// A CTA takes 8 rows of a row block and 32 kQuads of its 128 column quads: thread
-// i the row i % 8, so that 8 rows of a quad are read as one line.  The grid has a
-// slice for every row block or, where those are more, for every boundary between
-// pairs: then the row block whose first cut the boundary is.
+// A CTA takes 8 rows of a row block and kMergeColumns / kStreams x kQuads of its
+// 128 column quads: thread i the row i % 8, so that 8 rows of a quad are read as
+// one line, and one partial of kStreams.  The grid has a slice for every row block
+// or, where those are more, for every boundary between pairs: then the row block
+// whose first cut the boundary is.
 constexpr int kMergeRows = 8, kMergeColumns = 32;
 
-template <int kQuads, int kAhead>  // kAhead: partials whose loads are in flight together
+template <int kQuads, int kAhead, int kStreams>  // kAhead: partials whose loads are in flight together
 __global__ void __launch_bounds__(kMergeRows * kMergeColumns)
     dsa_prefix_merge_kernel(const PrefixParams p, const int by_cut) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -819,16 +820,17 @@ __global__ void __launch_bounds__(kMergeRows * kMergeColumns)
     began_before = deal.start(first) < c0;
   }
   if (first == last) return;  // one pair had it all and wrote the results
-  constexpr int kParts = 128 / (kMergeColumns * kQuads);
+  constexpr int kWide = kMergeColumns / kStreams, kParts = 128 / (kWide * kQuads);
+  const int column = threadIdx.x / kMergeRows, stream = column / kWide;
   const int row = blockIdx.x / kParts * kMergeRows + threadIdx.x % kMergeRows;
-  const int quad = blockIdx.x % kParts * (kMergeColumns * kQuads) + threadIdx.x / kMergeRows;
+  const int quad = blockIdx.x % kParts * (kWide * kQuads) + column % kWide;
   const int group = lo * kGroups + (row >> 4);
   if (group >= p.groups) return;
   float m = -INFINITY, l = 0.f;
   float4 o[kQuads];
 #pragma unroll
   for (int j = 0; j < kQuads; ++j) o[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int k0 = first; k0 <= last; k0 += kAhead) {
+  for (int k0 = first + stream; k0 <= last; k0 += kAhead * kStreams) {
     float mk[kAhead], lk[kAhead];
     float4 v[kAhead][kQuads];
 #pragma unroll
@@ -837,15 +839,16 @@ __global__ void __launch_bounds__(kMergeRows * kMergeColumns)
       lk[i] = 0.f;
 #pragma unroll
       for (int j = 0; j < kQuads; ++j) v[i][j] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (k0 + i <= last) {
+      const int k = k0 + i * kStreams;
+      if (k <= last) {
         // a pair that began before the block has it as its last, any other as its first
-        const int slot = 2 * (k0 + i) + (k0 + i == first && began_before);
+        const int slot = 2 * k + (k == first && began_before);
         const float* part = p.parts + (int64_t)slot * kSlotFloats;
         mk[i] = __ldcg(part + 2 * kRows * 512 + row);
         lk[i] = __ldcg(part + 2 * kRows * 512 + 2 * kRows + row);
 #pragma unroll
         for (int j = 0; j < kQuads; ++j)
-          v[i][j] = __ldcg(reinterpret_cast<const float4*>(part) + (quad + kMergeColumns * j) * (2 * kRows) + row);
+          v[i][j] = __ldcg(reinterpret_cast<const float4*>(part) + (quad + kWide * j) * (2 * kRows) + row);
       }
     }
     float top = m;
@@ -869,12 +872,30 @@ __global__ void __launch_bounds__(kMergeRows * kMergeColumns)
       }
     }
   }
+  if (kStreams > 1) {  // rows of a CTA are of one group: all its threads are here
+    __shared__ float4 all_o[kStreams > 1 ? kMergeRows * kMergeColumns : 1];
+    __shared__ float2 all_ml[kStreams > 1 ? kMergeRows * kMergeColumns : 1];
+    all_o[threadIdx.x] = o[0];
+    all_ml[threadIdx.x] = make_float2(m, l);
+    __syncthreads();
+    if (stream > 0) return;
+    for (int s = 1; s < kStreams; ++s) {
+      const int at = threadIdx.x + s * kWide * kMergeRows;
+      const float2 ml = all_ml[at];
+      const float top = fmaxf(m, ml.x);
+      const float a = m == -INFINITY ? 0.f : exp2f(m - top), b = ml.x == -INFINITY ? 0.f : exp2f(ml.x - top);
+      m = top;
+      l = l * a + ml.y * b;
+      o[0] = make_float4(o[0].x * a + all_o[at].x * b, o[0].y * a + all_o[at].y * b, o[0].z * a + all_o[at].z * b,
+                         o[0].w * a + all_o[at].w * b);
+    }
+  }
   const int token = (unsigned)group / (unsigned)p.group_per_token;
   const int head = (group - token * p.group_per_token) * 16 + (row & 15);
   const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
   for (int j = 0; j < kQuads; ++j)
-    *reinterpret_cast<uint2*>(p.out + token * p.out_st + head * p.out_sh + (quad + kMergeColumns * j) * 4) =
+    *reinterpret_cast<uint2*>(p.out + token * p.out_st + head * p.out_sh + (quad + kWide * j) * 4) =
         make_uint2(pack_bf16(o[j].x * inv, o[j].y * inv), pack_bf16(o[j].z * inv, o[j].w * inv));
   if (quad == 0) p.lse[token * p.lse_st + head * p.lse_sh] = l == 0.f ? -INFINITY : m + log2f(l);
 }
@@ -1095,11 +1116,14 @@ extern "C" int dsa_shared_prefix_attention(
   if (e == cudaSuccess && pairs > 1 && !whole) {
     const int rows = (p.groups < kGroups ? p.groups : kGroups) * 16, by_cut = p.blocks >= pairs;
     const unsigned x = rows / kMergeRows, y = (unsigned)(by_cut ? pairs - 1 : p.blocks), threads = kMergeRows * kMergeColumns;
-    // few row blocks have many partials each: more threads, each with more of them in flight
-    if (x * y <= 148)
-      e = launch_after(dsa_prefix_merge_kernel<1, 8>, dim3(4 * x, y), threads, 0, s, p, by_cut);
+    // few row blocks have many partials each: more of them in flight, and over 16
+    // dealt out to 8 threads (a token behind 131072 rows, 74 partials: 56 -> 42 us a call)
+    if (pairs / p.blocks > 16)
+      e = launch_after(dsa_prefix_merge_kernel<1, 5, 8>, dim3(32 * x, y), threads, 0, s, p, by_cut);
+    else if (x * y <= 148)
+      e = launch_after(dsa_prefix_merge_kernel<1, 10, 1>, dim3(4 * x, y), threads, 0, s, p, by_cut);
     else
-      e = launch_after(dsa_prefix_merge_kernel<4, 2>, dim3(x, y), threads, 0, s, p, by_cut);
+      e = launch_after(dsa_prefix_merge_kernel<4, 2, 1>, dim3(x, y), threads, 0, s, p, by_cut);
   }
   if (e != cudaSuccess) return report_error(DSA_ERR_CUDA, cudaGetErrorString(e));
   return DSA_OK;
