@@ -737,33 +737,55 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       named_bar_sync(1, kSoftmaxThreads);  // red is written again by the next tile
       const int head = live ? (group - token * p.group_per_token) * 16 + (row & 15) : 0;
       const int dv = half * 256 + page * 128;  // the 128 columns of O in these lanes
-      float* part = p.parts + (int64_t)g.slot * kSlotFloats;
-      const bool whole = g.whole;
-      const float inv = l == 0.f ? 0.f : 1.f / l;
+      if (g.whole) {
+        // A lane holds a row, and 32 rows of 16 bytes are 32 lines a store: the warp
+        // turns 32 x 32 values over in its part of the idle weight buffer, so that
+        // four lanes store 64 bytes of a row (4 stores of 8 lines instead of 32).
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        uint8_t* stage = S.p[0] + warp * 2048;
+        const int chunk = lane & 3;
+        __nv_bfloat16* dst[2];  // of the two 16-head groups of the warp's rows
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        float o[32];
-        __syncwarp();
-        tmem_ld32(lanes + half * 128 + c * 32, o);
-        if (!live) continue;
-        if (whole) {
-          uint4* dst = reinterpret_cast<uint4*>(p.out + token * p.out_st + head * p.out_sh + dv + c * 32);
+        for (int i = 0; i < 2; ++i) {
+          const int its = g.block * kGroups + rank * 4 + (quarter & 1) * 2 + i;
+          const int t = (unsigned)its / (unsigned)p.group_per_token, h = (its - t * p.group_per_token) * 16;
+          dst[i] = its < p.groups ? p.out + t * p.out_st + (h + (lane >> 2)) * p.out_sh + dv + chunk * 8 : nullptr;
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          float o[32];
+          __syncwarp();
+          tmem_ld32(lanes + half * 128 + c * 32, o);
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            dst[j] = make_uint4(pack_bf16(o[8 * j] * inv, o[8 * j + 1] * inv), pack_bf16(o[8 * j + 2] * inv, o[8 * j + 3] * inv),
-                                pack_bf16(o[8 * j + 4] * inv, o[8 * j + 5] * inv), pack_bf16(o[8 * j + 6] * inv, o[8 * j + 7] * inv));
-        } else {
-          // partials lie as [512 / 4][128 rows][4]: the lanes of a warp store side by side
+            *reinterpret_cast<uint4*>(stage + lane * 64 + ((j ^ (lane >> 1 & 3)) << 4)) =
+                make_uint4(pack_bf16(o[8 * j] * inv, o[8 * j + 1] * inv), pack_bf16(o[8 * j + 2] * inv, o[8 * j + 3] * inv),
+                           pack_bf16(o[8 * j + 4] * inv, o[8 * j + 5] * inv), pack_bf16(o[8 * j + 6] * inv, o[8 * j + 7] * inv));
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {  // rows 8 k + lane / 4
+            const int r = 8 * k + (lane >> 2);
+            const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 64 + ((chunk ^ (r >> 1 & 3)) << 4));
+            if (dst[k >> 1]) *reinterpret_cast<uint4*>(dst[k >> 1] + (k & 1) * 8 * p.out_sh + c * 32) = v;
+          }
+        }
+        if (live && half == 0 && page == 0)
+          p.lse[token * p.lse_st + head * p.lse_sh] = l == 0.f ? -INFINITY : m + log2f(l);
+      } else {
+        // partials lie as [512 / 4][128 rows][4]: the lanes of a warp store side by side
+        float* part = p.parts + (int64_t)g.slot * kSlotFloats;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          float o[32];
+          __syncwarp();
+          tmem_ld32(lanes + half * 128 + c * 32, o);
+          if (!live) continue;
           float4* dst = reinterpret_cast<float4*>(part) + (dv + c * 32) / 4 * (2 * kRows) + rank * kRows + row;
 #pragma unroll
           for (int j = 0; j < 8; ++j)
             __stcg(dst + j * (2 * kRows), make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]));
         }
-      }
-      if (live && half == 0 && page == 0) {
-        if (whole) {
-          p.lse[token * p.lse_st + head * p.lse_sh] = l == 0.f ? -INFINITY : m + log2f(l);
-        } else {
+        if (live && half == 0 && page == 0) {
           __stcg(part + 2 * kRows * 512 + rank * kRows + row, m);
           __stcg(part + 2 * kRows * 512 + 2 * kRows + rank * kRows + row, l);
         }
