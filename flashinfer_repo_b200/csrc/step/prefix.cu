@@ -25,9 +25,9 @@
 // the end of the tile and has the TMA write zeros before them.
 //
 // Bound by the MMA: 2186 cycles a tile alone, 2510-2800 here.  128 tokens of 128
-// heads behind 16384 rows: 470 us, 1.25 PFLOP/s at the clock that the power limit
-// leaves (92% of what a cuBLAS product sustains); 64 tokens of 16 heads behind
-// 32768 rows: 64-80 us, 20 of them the plan, the first loads, partials and merge.
+// heads behind 16384 rows: 458 us, 1.29 PFLOP/s at the clock that the power limit
+// leaves (94% of what a cuBLAS product sustains); 64 tokens of 16 heads behind
+// 32768 rows: 64-79 us, 20 of them the plan, the first loads, partials and merge.
 #include <cuda.h>
 
 #include <mutex>

@@ -354,8 +354,8 @@ int dsa_step_layout(const int32_t* seq_lens, const int32_t* query_lens, int64_t 
  * inverse != 0 turns back, which with the same scale is also the gradient.
  * Strides are in elements, the last dimension is contiguous; out may be x (then
  * only the slice is written) but must not overlap it in another way.  rot_dim is
- * even, at most 512; a token has at most 2^28 values.  positions are int32 or int64.  No counterpart in the
- * reference, which takes rotated queries and keys.
+ * even, at most 512; a token has at most 2^28 values.  positions are int32 or
+ * int64.  No counterpart in the reference, which takes rotated queries and keys.
  */
 int dsa_apply_rope(const void* x, int64_t x_stride_token, int64_t x_stride_head, void* out,
                    int64_t out_stride_token, int64_t out_stride_head, int dtype, int64_t num_tokens,
