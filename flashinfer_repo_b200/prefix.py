@@ -75,7 +75,8 @@ def shared_prefix_attention(q_nope, q_pe, ckv_cache, kpe_cache, prefix_pages, pr
     tensor of prefix_workspace_size(T, H) bytes for calls that may run at the
     same time as others on the device (the default one is shared, so such calls
     must not overlap).  Errors found on the device (page ids or requests outside
-    their range: those rows are skipped) are read by `read_prefix_error`.
+    their range: those rows are skipped) are read by `read_prefix_error`, those of
+    calls with a workspace of their own in its first int32.
     """
     tokens, heads, dim = q_nope.shape
     num_pages = ckv_cache.shape[0]
