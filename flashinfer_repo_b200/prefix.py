@@ -105,7 +105,7 @@ def shared_prefix_attention(q_nope, q_pe, ckv_cache, kpe_cache, prefix_pages, pr
     else:
         assert requests >= tokens, "without token_request the block table needs a row for every token"
     if output is None:
-        output = q_nope.new_empty((tokens, heads, HEAD_DIM_CKV))
+        output = torch.empty_like(q_nope, memory_format=torch.contiguous_format)
         out_token, out_head = heads * HEAD_DIM_CKV, HEAD_DIM_CKV
     else:
         assert output.shape == (tokens, heads, HEAD_DIM_CKV) and output.dtype == bf16
