@@ -13,7 +13,7 @@
 namespace dsa {
 namespace {
 
-constexpr int kLatent = 512, kRot = 64;
+constexpr int kLatent = 512;
 
 struct AppendParams {
   const void* kv;
