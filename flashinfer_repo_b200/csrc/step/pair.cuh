@@ -63,6 +63,15 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity
     if (clock64() - t0 > kWaitBudgetCycles) return false;
   }
 }
+// The same two waits by a whole warp: every lane polls for itself, and the vote
+// brings the warp together again, as the .aligned instructions behind a wait
+// demand, and lets its lanes agree where the clock budget ran out for some.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity));
+}
+__device__ __forceinline__ bool mbar_wait_cluster_warp(uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, mbar_wait_cluster(bar, parity));
+}
 // Arrivals on a barrier given by its shared::cluster address (own or the other
 // CTA's).  The first orders this thread's shared-memory accesses at CTA scope:
 // enough for data that the pair's MMA reads on the writer's own SM, once

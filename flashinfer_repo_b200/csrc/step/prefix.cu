@@ -319,7 +319,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     if (rank == 0 && lane == 0 && u < u1) p.begins[pair] = block;
     for (int n = 0;; ++n) {
       const int s = n & 1;
-      if (!mbar_wait(&S.seg_empty[s], ((n >> 1) & 1) ^ 1)) {
+      if (!mbar_wait_warp(&S.seg_empty[s], ((n >> 1) & 1) ^ 1)) {
         set_error(p.err, kErrTimeout);
         break;
       }
@@ -407,7 +407,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     int it = 0;
     for (int n = 0; ok; ++n) {
       const Segment& g = S.seg[n & 1];
-      if (!mbar_wait(&S.seg_full[n & 1], (n >> 1) & 1)) {
+      if (!mbar_wait_warp(&S.seg_full[n & 1], (n >> 1) & 1)) {
         ok = false;
         break;
       }
@@ -432,7 +432,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       // queries: of the first segment by the warp that waits longest for its own
       // loads, later by the one that sees the queries' last use first
       if (keys == (n > 0)) {
-        if (!mbar_wait(&S.q_empty, (n & 1) ^ 1)) {
+        if (!mbar_wait_warp(&S.q_empty, (n & 1) ^ 1)) {
           ok = false;
           break;
         }
@@ -477,7 +477,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           const int my_page = rank ? page[1] : page[0], my_row = rank ? row[1] : row[0];
 #pragma unroll
           for (int c = 0; c < 3; ++c) {
-            if (!mbar_wait(&S.k_empty[c], parity)) {
+            if (!mbar_wait_warp(&S.k_empty[c], parity)) {
               ok = false;
               break;
             }
@@ -496,7 +496,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         } else {
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            if (!mbar_wait(&S.v_empty[c], parity)) {
+            if (!mbar_wait_warp(&S.v_empty[c], parity)) {
               ok = false;
               break;
             }
@@ -531,10 +531,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       uint32_t off[2][4];  // lanes left alone by the two pages of the tile before
       bool masked = false;
       auto weigh = [&](int i) -> bool {  // O += P V of tile i
-        if (!mbar_wait_cluster(&S.p_full, i & 1)) return false;
+        if (!mbar_wait_cluster_warp(&S.p_full, i & 1)) return false;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          if (!mbar_wait_cluster(&S.v_full[c], i & 1)) return false;
+          if (!mbar_wait_cluster_warp(&S.v_full[c], i & 1)) return false;
           tc_fence_after();
           if (elect_one()) {
             if (masked) {
@@ -558,7 +558,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       };
       for (int n = 0; ok; ++n) {
         const Segment& g = S.seg[n & 1];
-        if (!mbar_wait(&S.seg_full[n & 1], (n >> 1) & 1)) {
+        if (!mbar_wait_warp(&S.seg_full[n & 1], (n >> 1) & 1)) {
           ok = false;
           break;
         }
@@ -570,7 +570,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const int count = __shfl_sync(0xffffffffu, g.count, 0);
         if (count <= 0) break;
         int span = 0;
-        if (!mbar_wait_cluster(&S.q_full, n & 1)) {
+        if (!mbar_wait_cluster_warp(&S.q_full, n & 1)) {
           ok = false;
           break;
         }
@@ -578,7 +578,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           const uint32_t scores = base + kTmemS + 64 * (it & 1);
 #pragma unroll
           for (int c = 0; c < 3; ++c) {
-            if (!mbar_wait_cluster(&S.k_full[c], it & 1)) {
+            if (!mbar_wait_cluster_warp(&S.k_full[c], it & 1)) {
               ok = false;
               break;
             }
@@ -631,11 +631,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const int row = (quarter & 1) * 32 + lane;
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
     const uint32_t p_bar = cluster_map(smem_u32(&S.p_full), 0);
-    bool ok = true;  // a wait that gave up takes all eight warps out at their next barrier
+    // a wait that gave up in one warp takes all eight out at their next barrier, and
+    // nowhere else: a warp that left alone would keep the others waiting there
+    bool ok = true, left = false;
     int it = 0;
     for (int n = 0;; ++n) {
       const Segment& g = S.seg[n & 1];
-      ok = mbar_wait(&S.seg_full[n & 1], (n >> 1) & 1);
+      ok = mbar_wait_warp(&S.seg_full[n & 1], (n >> 1) & 1);
       if (!named_bar_all(1, kSoftmaxThreads, ok)) break;
       const int count = g.count;
       if (count <= 0) break;
@@ -648,7 +650,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       int span = 0;
       for (int i = 0; i < count; ++i, ++it) {
         const int k = 2 * (g.tile0 + i) + page;
-        ok = ok && mbar_wait(&S.valid_full[it & 3], (it >> 2) & 1) && mbar_wait_cluster(&S.s_full[it & 1], (it >> 1) & 1);
+        // ok is the same in all lanes of a warp: the votes of the waits are taken by all or none
+        ok = ok && mbar_wait_warp(&S.valid_full[it & 3], (it >> 2) & 1) && mbar_wait_cluster_warp(&S.s_full[it & 1], (it >> 1) & 1);
         tc_fence_after();
         bool sees = true;  // rows behind the last token see all: their queries are zeros and nobody reads them
         if (k >= g.pre_pages && k < g.pages) {
@@ -674,7 +677,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int j = 0; j < 16; ++j) top = fmaxf(top, fmaxf(x[j].x, x[j].y));
         S.red[it & 1][page * 2 + half][row] = top;
-        if (!(ok = named_bar_all(1, kSoftmaxThreads, ok))) break;
+        if ((left = !named_bar_all(1, kSoftmaxThreads, ok))) break;
         top = p.scale_log2 * fmaxf(fmaxf(S.red[it & 1][0][row], S.red[it & 1][1][row]),
                                    fmaxf(S.red[it & 1][2][row], S.red[it & 1][3][row]));
         // the maximum moves on a rise of more than 2^kLazy only (weights up to
@@ -697,7 +700,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
 #pragma unroll
         for (int j = 0; j < 16; ++j) asm volatile("" : "+r"(w[j]));  // done before the wait, not behind it
-        if (it > 0) ok = mbar_wait_cluster(&S.pv_done, (it - 1) & 1);  // P is read, O settled
+        if (it > 0) ok = mbar_wait_cluster_warp(&S.pv_done, (it - 1) & 1);  // P is read, O settled
+        __syncwarp();  // of one mind for the accesses to TMEM, whichever way the lanes came
         tc_fence_after();
         if (i == 0) {
           float z[32];
@@ -726,14 +730,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive_at(p_bar);
       }
-      if (!ok) break;
+      if (left) {
+        ok = false;
+        break;
+      }
       // the four threads of a row add up their sums; O is complete
       float l = sums.x + sums.y;
       S.red[it & 1][page * 2 + half][row] = l;
-      ok = mbar_wait_cluster(&S.pv_done, (it - 1) & 1);
+      ok = ok && mbar_wait_cluster_warp(&S.pv_done, (it - 1) & 1);
       if (!(ok = named_bar_all(1, kSoftmaxThreads, ok))) break;
       tc_fence_after();
       l = S.red[it & 1][0][row] + S.red[it & 1][1][row] + S.red[it & 1][2][row] + S.red[it & 1][3][row];
+      __syncwarp();
       named_bar_sync(1, kSoftmaxThreads);  // red is written again by the next tile
       const int head = live ? (group - token * p.group_per_token) * 16 + (row & 15) : 0;
       const int dv = half * 256 + page * 128;  // the 128 columns of O in these lanes
