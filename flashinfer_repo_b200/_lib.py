@@ -64,6 +64,9 @@ SIGNATURES = {
     "dsa_shared_prefix_attention": [P, I64, I64, P, I64, I64, P, I64, I64, P, I64, I64, P, I64, P, P, I64,
                                     I64, I64, P, P, I64, I64, I64, F32, P, I64, I64, P, I64, I64, P, SZ,
                                     P],
+    "dsa_shared_prefix_attention_scratch": [P, I64, I64, P, I64, I64, P, I64, I64, P, I64, I64, P, I64, P, P,
+                                            I64, I64, I64, P, P, I64, I64, I64, F32, P, I64, I64, P, I64, I64,
+                                            P, SZ, P, P],
 }
 
 
@@ -128,6 +131,31 @@ def call_on(index: int, fn_name: str, *args):
             rc = f(*args, _current_stream(index))
     if rc != 0:
         check(fn_name, rc)
+
+
+# memory of torch's allocator without a tensor around it: 0.5 us, a tensor takes 1.6
+_alloc = getattr(torch._C, "_cuda_cudaCachingAllocator_raw_alloc", None)
+_free = getattr(torch._C, "_cuda_cudaCachingAllocator_raw_delete", None)
+
+
+def call_with_scratch(index: int, fn_name: str, nbytes: int, error: int, *args):
+    """`call_on` of a function whose last arguments are a workspace, its size, a
+    device error word and the stream.  The workspace is torch's memory of that
+    stream (of the graph, in a capture) and goes back to it in stream order."""
+    if _current_device() != index:
+        with torch.cuda.device(index):
+            return call_with_scratch(index, fn_name, nbytes, error, *args)
+    stream = _current_stream(index)
+    f = _bound.get(fn_name)
+    if f is None:
+        f = _bound[fn_name] = getattr(load(), fn_name)
+    scratch = _alloc(nbytes, stream)
+    try:
+        rc = f(*args, scratch, nbytes, error, stream)
+        if rc != 0:
+            check(fn_name, rc)
+    finally:
+        _free(scratch)
 
 
 def same_device(first, *others) -> int:

@@ -1037,7 +1037,7 @@ extern "C" int dsa_shared_prefix_attention_workspace_size(int64_t num_tokens, in
   return DSA_OK;
 }
 
-extern "C" int dsa_shared_prefix_attention(
+extern "C" int dsa_shared_prefix_attention_scratch(
     const void* q_nope, int64_t q_nope_stride_token, int64_t q_nope_stride_head, const void* q_pe,
     int64_t q_pe_stride_token, int64_t q_pe_stride_head, const void* ckv_cache, int64_t ckv_stride_page,
     int64_t ckv_stride_row, const void* kpe_cache, int64_t kpe_stride_page, int64_t kpe_stride_row,
@@ -1045,7 +1045,7 @@ extern "C" int dsa_shared_prefix_attention(
     int64_t block_table_stride, int64_t batch, int64_t max_pages, const int32_t* token_request,
     const int32_t* token_lens, int64_t num_tokens, int64_t num_heads, int64_t num_pages, float sm_scale,
     void* output, int64_t out_stride_token, int64_t out_stride_head, float* lse, int64_t lse_stride_token,
-    int64_t lse_stride_head, void* workspace, size_t workspace_bytes, void* stream) {
+    int64_t lse_stride_head, void* workspace, size_t workspace_bytes, int* device_error, void* stream) {
   if (num_tokens < 0 || max_prefix_len < 0 || batch < 0 || max_pages < 0 || num_pages < 0)
     return report_error(DSA_ERR_INVALID_ARG, "negative size");
   if (num_heads <= 0 || num_heads % 16)
@@ -1139,7 +1139,7 @@ extern "C" int dsa_shared_prefix_attention(
   p.lse = lse;
   p.lse_st = lse_stride_token;
   p.lse_sh = lse_stride_head;
-  p.err = static_cast<int*>(workspace);
+  p.err = device_error;
   p.cum = reinterpret_cast<long long*>(static_cast<char*>(workspace) + w.cum);
   p.begins = reinterpret_cast<int*>(static_cast<char*>(workspace) + w.begins);
   p.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + w.parts);
@@ -1160,4 +1160,21 @@ extern "C" int dsa_shared_prefix_attention(
   }
   if (e != cudaSuccess) return report_error(DSA_ERR_CUDA, cudaGetErrorString(e));
   return DSA_OK;
+}
+
+extern "C" int dsa_shared_prefix_attention(
+    const void* q_nope, int64_t q_nope_stride_token, int64_t q_nope_stride_head, const void* q_pe,
+    int64_t q_pe_stride_token, int64_t q_pe_stride_head, const void* ckv_cache, int64_t ckv_stride_page,
+    int64_t ckv_stride_row, const void* kpe_cache, int64_t kpe_stride_page, int64_t kpe_stride_row,
+    const int32_t* prefix_pages, int64_t max_prefix_len, const int32_t* prefix_len, const int32_t* block_table,
+    int64_t block_table_stride, int64_t batch, int64_t max_pages, const int32_t* token_request,
+    const int32_t* token_lens, int64_t num_tokens, int64_t num_heads, int64_t num_pages, float sm_scale,
+    void* output, int64_t out_stride_token, int64_t out_stride_head, float* lse, int64_t lse_stride_token,
+    int64_t lse_stride_head, void* workspace, size_t workspace_bytes, void* stream) {
+  return dsa_shared_prefix_attention_scratch(
+      q_nope, q_nope_stride_token, q_nope_stride_head, q_pe, q_pe_stride_token, q_pe_stride_head, ckv_cache,
+      ckv_stride_page, ckv_stride_row, kpe_cache, kpe_stride_page, kpe_stride_row, prefix_pages, max_prefix_len,
+      prefix_len, block_table, block_table_stride, batch, max_pages, token_request, token_lens, num_tokens, num_heads,
+      num_pages, sm_scale, output, out_stride_token, out_stride_head, lse, lse_stride_token, lse_stride_head, workspace,
+      workspace_bytes, static_cast<int*>(workspace), stream);
 }

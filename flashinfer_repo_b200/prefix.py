@@ -16,7 +16,7 @@ import torch
 from . import _lib
 from .kernel import HEAD_DIM_CKV, HEAD_DIM_KPE, NUM_HEADS, PAGE_SIZE
 
-_workspaces: dict[int, list] = {}  # per device: every buffer handed out, the newest last
+_workspaces: dict[int, torch.Tensor] = {}  # per device: the word that collects device errors
 _lock = threading.Lock()
 _size_cache: dict[tuple, int] = {}
 
@@ -41,20 +41,21 @@ def _index(device) -> int:
     return index if index is not None else torch.cuda.current_device()
 
 
-def _workspace(index: int, nbytes: int) -> torch.Tensor:
-    """The device's shared workspace.  Few calls outgrow it (its size hardly
-    depends on the shape); they get a new one, and the old one is kept, since a
-    captured graph may hold its address."""
-    kept = _workspaces.get(index)
-    if not kept or kept[-1].numel() < nbytes:
+def _error_word(index: int) -> torch.Tensor:
+    """The device's error word for calls without a workspace of their own.  It
+    stays, since a captured graph may hold its address."""
+    word = _workspaces.get(index)
+    if word is None:
         with _lock, torch.cuda.device(index):
-            kept = _workspaces.setdefault(index, [])
-            if not kept or kept[-1].numel() < nbytes:
+            word = _workspaces.get(index)
+            if word is None:
                 if torch.cuda.is_current_stream_capturing():
-                    raise RuntimeError("the workspace must grow during stream capture: make one call of this size "
-                                       "before the capture, or pass workspace=")
-                kept.append(torch.zeros(nbytes + (4 << 20), dtype=torch.uint8, device=f"cuda:{index}"))
-    return kept[-1]
+                    raise RuntimeError("the error word cannot be made during stream capture: make one call on the "
+                                       "device before the capture, or pass workspace=")
+                word = torch.zeros(64, dtype=torch.int32, device=f"cuda:{index}")
+                torch.cuda.current_stream().synchronize()  # zero before a call on another stream can set it
+                _workspaces[index] = word
+    return word
 
 
 def shared_prefix_attention(q_nope, q_pe, ckv_cache, kpe_cache, prefix_pages, prefix_len, block_table, token_lens,
@@ -71,12 +72,14 @@ def shared_prefix_attention(q_nope, q_pe, ckv_cache, kpe_cache, prefix_pages, pr
     `step_layout` makes token_lens and token_request.  A token that sees no row
     gets output 0 and lse -inf.  Rows past a length are never read.
 
-    output/lse write into existing tensors.  workspace: a zeroed uint8 CUDA
-    tensor of prefix_workspace_size(T, H) bytes for calls that may run at the
-    same time as others on the device (the default one is shared, so such calls
-    must not overlap).  Errors found on the device (page ids or requests outside
-    their range: those rows are skipped) are read by `read_prefix_error`, those of
-    calls with a workspace of their own in its first int32.
+    output/lse write into existing tensors.  Plan and partials take about 40 MB
+    of torch's memory for the time of the call, so calls on several streams or
+    threads and captured graphs do not meet (the first call on a device must not
+    be a captured one).  workspace: a zeroed, 256-byte aligned uint8 CUDA tensor of
+    prefix_workspace_size(T, H) bytes to use instead; calls that share it must not
+    overlap.  Errors found on the device (page ids or requests outside their
+    range: those rows are skipped) are read by `read_prefix_error`, those of calls
+    with a workspace of their own in its first int32.
     """
     tokens, heads, dim = q_nope.shape
     num_pages = ckv_cache.shape[0]
@@ -128,17 +131,18 @@ def shared_prefix_attention(q_nope, q_pe, ckv_cache, kpe_cache, prefix_pages, pr
     rows_c, c_page, c_row = _tiled(ckv_cache)
     rows_e, e_page, e_row = _tiled(kpe_cache)
     assert rows_c is ckv_cache and rows_e is kpe_cache, "cache rows must be contiguous, 16-byte aligned and apart"
+    args = (q_nope.data_ptr(), qn_token, qn_head, q_pe.data_ptr(), qp_token, qp_head, ckv_cache.data_ptr(), c_page, c_row,
+            kpe_cache.data_ptr(), e_page, e_row, prefix_pages.data_ptr(), bound,
+            length.data_ptr() if length is not None else None, block_table.data_ptr(), block_table.stride(0), requests,
+            width, token_request.data_ptr() if token_request is not None else None, token_lens.data_ptr(), tokens, heads,
+            num_pages, sm_scale, output.data_ptr(), out_token, out_head, lse.data_ptr(), lse_token, lse_head)
     if workspace is None:
-        workspace = _workspace(index, prefix_workspace_size(tokens, heads, index))
-    elif not (workspace.dtype == torch.uint8 and workspace.is_contiguous()):
+        _lib.call_with_scratch(index, "dsa_shared_prefix_attention_scratch", prefix_workspace_size(tokens, heads, index),
+                               _error_word(index).data_ptr(), *args)
+    elif workspace.dtype == torch.uint8 and workspace.is_contiguous():
+        _lib.call_on(index, "dsa_shared_prefix_attention", *args, workspace.data_ptr(), workspace.numel())
+    else:
         raise ValueError("workspace must be a contiguous uint8 tensor on the inputs' device")
-    _lib.call_on(index, "dsa_shared_prefix_attention", q_nope.data_ptr(), qn_token, qn_head, q_pe.data_ptr(), qp_token,
-                 qp_head, ckv_cache.data_ptr(), c_page, c_row, kpe_cache.data_ptr(), e_page, e_row,
-                 prefix_pages.data_ptr(), bound, length.data_ptr() if length is not None else None,
-                 block_table.data_ptr(), block_table.stride(0), requests, width,
-                 token_request.data_ptr() if token_request is not None else None, token_lens.data_ptr(), tokens,
-                 heads, num_pages, sm_scale, output.data_ptr(), out_token, out_head, lse.data_ptr(), lse_token,
-                 lse_head, workspace.data_ptr(), workspace.numel())
     return output, lse
 
 
@@ -157,14 +161,14 @@ def _tiled(t: torch.Tensor):
 
 
 def read_prefix_error(device=None, clear=True) -> int:
-    """Synchronise and return the DSA_DEVERR_* bits raised by
-    shared_prefix_attention calls that used the device's shared workspace."""
+    """Synchronise the current stream and return the DSA_DEVERR_* bits raised by
+    shared_prefix_attention calls without a workspace of their own."""
     index = _index(device)
-    bits = 0
+    word = _workspaces.get(index)
+    if word is None:
+        return 0
+    bits = ctypes.c_int(0)
     with torch.cuda.device(index):
-        stream = torch.cuda.current_stream().cuda_stream
-        for buf in _workspaces.get(index, []):
-            word = ctypes.c_int(0)
-            _lib.call("dsa_read_device_error", buf.data_ptr(), int(clear), ctypes.byref(word), stream)
-            bits |= word.value
-    return bits
+        _lib.call("dsa_read_device_error", word.data_ptr(), int(clear), ctypes.byref(bits),
+                  torch.cuda.current_stream().cuda_stream)
+    return bits.value

@@ -421,6 +421,23 @@ int dsa_shared_prefix_attention(
     size_t workspace_bytes, void* stream);
 
 /*
+ * The same with the device errors in a word of their own (device_error, NULL:
+ * not reported): the workspace is then scratch that need not be zeroed and holds
+ * nothing from one call to the next, so that every call can bring memory that
+ * belongs to its stream.
+ */
+int dsa_shared_prefix_attention_scratch(
+    const void* q_nope, int64_t q_nope_stride_token, int64_t q_nope_stride_head, const void* q_pe,
+    int64_t q_pe_stride_token, int64_t q_pe_stride_head, const void* ckv_cache, int64_t ckv_stride_page,
+    int64_t ckv_stride_row, const void* kpe_cache, int64_t kpe_stride_page, int64_t kpe_stride_row,
+    const int32_t* prefix_pages, int64_t max_prefix_len, const int32_t* prefix_len,
+    const int32_t* block_table, int64_t block_table_stride, int64_t batch, int64_t max_pages,
+    const int32_t* token_request, const int32_t* token_lens, int64_t num_tokens, int64_t num_heads,
+    int64_t num_pages, float sm_scale, void* output, int64_t out_stride_token, int64_t out_stride_head,
+    float* lse, int64_t lse_stride_token, int64_t lse_stride_head, void* workspace,
+    size_t workspace_bytes, int* device_error, void* stream);
+
+/*
  * Read (and optionally clear) the device error word of a workspace.
  * Synchronises the stream.  *bits receives DSA_DEVERR_* flags.
  */
