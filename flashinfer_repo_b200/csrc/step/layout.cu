@@ -136,6 +136,8 @@ __global__ void __launch_bounds__(kLayThreads) dsa_step_layout_kernel(const Layo
         if (have_it) page = col < have ? p.table[(b0 + b) * p.bt_stride + col] : p.free_pages[src];
         // a slot past 2^31 rows has no 32-bit id: no cache of this library is that long
         if (have_it && (page < 0 || page >= (1 << 25))) bits |= kErrBadIndex;
+      } else {
+        bits |= kErrCapacity;  // of a page that the request had before too, though none is handed out for it
       }
       const long long out = rows_base + i;
       const bool ok = page >= 0 && page < (1 << 25);

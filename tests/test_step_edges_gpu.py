@@ -1,0 +1,40 @@
+"""The serving-step operators at the edges of what their documentation allows."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import flashinfer_repo_b200 as fi
+
+from . import prefix_oracle as P
+
+pytestmark = pytest.mark.gpu
+SCALE = 1 / math.sqrt(192.0)
+I32 = torch.int32
+
+
+def _put(*v):
+    return torch.tensor(v, dtype=I32, device="cuda")
+
+
+def _attend(c, **kw):
+    a = {"pages": c["pages"], "prefix": c["prefix"], "ckv": c["ckv"], "kpe": c["kpe"], **kw}
+    extra = {k: a[k] for k in ("output", "lse", "workspace") if k in a}
+    return fi.shared_prefix_attention(c["qn"], c["qp"], a["ckv"], a["kpe"], a["pages"], a["prefix"], c["table"], c["lens"],
+                                      SCALE, token_request=c["request"], **extra)
+
+
+# ------------------------------------------------------------- step layout
+@pytest.mark.parametrize("seq,q,width,slots", [
+    (641, 1, 10, [-1]),            # the row's page is a column past the table and was there before
+    (700, 3, 8, [-1, -1, -1]),
+    (639, 2, 10, [5 * 64 + 63, -1]),  # the second row would need a new one past the table
+    (638, 2, 10, [5 * 64 + 62, 5 * 64 + 63])])
+def test_layout_flags_rows_past_the_table(seq, q, width, slots):
+    table = torch.full((1, width), 5, dtype=I32, device="cuda")
+    err = torch.zeros(1, dtype=I32, device="cuda")
+    lay = fi.step_layout(_put(seq), _put(q), table, _put(7, 8, 9), q, device_error=err)
+    assert lay.slots.tolist() == slots and err.item() == (4 if -1 in slots else 0)
+    assert (table == 5).all()
