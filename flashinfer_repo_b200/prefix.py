@@ -95,6 +95,7 @@ def shared_prefix_attention(q_nope, q_pe, ckv_cache, kpe_cache, prefix_pages, pr
         "queries and caches must be bfloat16"
     requests, width = block_table.shape
     assert token_lens.shape == (tokens,), "token_lens must be [tokens]"
+    assert prefix_pages.dim() == 1, "prefix_pages must be one list of pages"
     prefix_pages, token_lens = _lib.int32(prefix_pages, "prefix_pages"), _lib.int32(token_lens, "token_lens")
     if length is not None:
         assert length.numel() == 1 and length.dtype == torch.int32, "prefix_len must be an int or one int32"

@@ -38,3 +38,12 @@ def test_layout_flags_rows_past_the_table(seq, q, width, slots):
     lay = fi.step_layout(_put(seq), _put(q), table, _put(7, 8, 9), q, device_error=err)
     assert lay.slots.tolist() == slots and err.item() == (4 if -1 in slots else 0)
     assert (table == 5).all()
+
+
+# ------------------------------------------------------ shared-prefix attention
+def test_prefix_pages_must_be_one_list():
+    c = P.make_case(1, 3, 16, 200, [1, 0, 70])
+    for pages in (c["pages"][None], c["pages"][:, None]):
+        for prefix in (c["prefix"], 64):
+            with pytest.raises(AssertionError, match="prefix_pages"):
+                _attend(c, pages=pages, prefix=prefix)
