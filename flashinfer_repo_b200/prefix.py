@@ -116,12 +116,14 @@ def shared_prefix_attention(q_nope, q_pe, ckv_cache, kpe_cache, prefix_pages, pr
         out_token, out_head, last = output.stride()
         assert last == 1 and out_token % 8 == 0 and out_head % 8 == 0 and output.data_ptr() % 16 == 0, \
             "output rows must be contiguous and 16-byte aligned"
+        assert (out_token > 0 or tokens <= 1) and out_head > 0, "output is an expanded tensor"
     if lse is None:
         lse = q_nope.new_empty((tokens, heads), dtype=torch.float32)
         lse_token, lse_head = heads, 1
     else:
         assert lse.shape == (tokens, heads) and lse.dtype == torch.float32
         lse_token, lse_head = lse.stride()
+        assert (lse_token > 0 or tokens <= 1) and lse_head > 0, "lse is an expanded tensor"
     if tokens == 0:
         return output, lse
     assert num_pages > 0, "the cache has no pages"

@@ -47,3 +47,19 @@ def test_prefix_pages_must_be_one_list():
         for prefix in (c["prefix"], 64):
             with pytest.raises(AssertionError, match="prefix_pages"):
                 _attend(c, pages=pages, prefix=prefix)
+
+
+def test_outputs_shared_by_rows_are_refused():
+    c = P.make_case(2, 3, 32, 100, [1, 0, 70])
+    for output in (torch.empty((1, 32, 512), dtype=torch.bfloat16, device="cuda").expand(3, 32, 512),
+                   torch.empty((3, 1, 512), dtype=torch.bfloat16, device="cuda").expand(3, 32, 512)):
+        with pytest.raises(AssertionError, match="expanded"):
+            _attend(c, output=output)
+    for lse in (torch.empty((1, 32), device="cuda").expand(3, 32), torch.empty((3, 1), device="cuda").expand(3, 32)):
+        with pytest.raises(AssertionError, match="expanded"):
+            _attend(c, lse=lse)
+    # a single token or any strides that keep rows apart are fine
+    one = {**c, "qn": c["qn"][:1], "qp": c["qp"][:1], "lens": c["lens"][:1], "request": c["request"][:1]}
+    P.check(one, _attend(one, output=torch.empty((1, 32, 512), dtype=torch.bfloat16, device="cuda").expand(1, 32, 512)), SCALE)
+    turned = torch.empty((32, 3, 512), dtype=torch.bfloat16, device="cuda").transpose(0, 1)
+    P.check(c, _attend(c, output=turned, lse=torch.empty((32, 3), device="cuda").T), SCALE)
