@@ -129,11 +129,11 @@ def shared_prefix_attention(q_nope, q_pe, ckv_cache, kpe_cache, prefix_pages, pr
     assert num_pages > 0, "the cache has no pages"
     if block_table.dtype != torch.int32 or (width > 1 and block_table.stride(1) != 1):
         block_table = _lib.int32(block_table, "block_table")
+    ckv_strides, kpe_strides = _tile_strides(ckv_cache), _tile_strides(kpe_cache)
+    assert ckv_strides and kpe_strides, "cache rows must be contiguous, 16-byte aligned and apart"
+    (c_page, c_row), (e_page, e_row) = ckv_strides, kpe_strides
     q_nope, qn_token, qn_head = _tiled(q_nope)
     q_pe, qp_token, qp_head = _tiled(q_pe)
-    rows_c, c_page, c_row = _tiled(ckv_cache)
-    rows_e, e_page, e_row = _tiled(kpe_cache)
-    assert rows_c is ckv_cache and rows_e is kpe_cache, "cache rows must be contiguous, 16-byte aligned and apart"
     args = (q_nope.data_ptr(), qn_token, qn_head, q_pe.data_ptr(), qp_token, qp_head, ckv_cache.data_ptr(), c_page, c_row,
             kpe_cache.data_ptr(), e_page, e_row, prefix_pages.data_ptr(), bound,
             length.data_ptr() if length is not None else None, block_table.data_ptr(), block_table.stride(0), requests,
@@ -149,18 +149,26 @@ def shared_prefix_attention(q_nope, q_pe, ckv_cache, kpe_cache, prefix_pages, pr
     return output, lse
 
 
-def _tiled(t: torch.Tensor):
-    """(t, outer, inner stride) of t [A, B, width] if the TMA can read its rows
-    where they are, else of a contiguous copy."""
+def _tile_strides(t: torch.Tensor):
+    """(outer, inner stride) of t [A, B, width] if the TMA can read its rows where
+    they are, else None."""
     if t.is_contiguous() and t.data_ptr() % 16 == 0:
         _, rows, width = t.shape
-        return t, rows * width, width
+        return rows * width, width
     outer, inner, last = t.stride()
     if last == 1 and inner % 8 == 0 and inner >= t.shape[2] and t.data_ptr() % 16 == 0 and (
             t.shape[0] == 1 or (outer >= inner and outer % 8 == 0)):
-        return t, outer, inner
-    t = t.clone(memory_format=torch.contiguous_format)
-    return t, t.stride(0), t.stride(1)
+        return outer, inner
+    return None
+
+
+def _tiled(t: torch.Tensor):
+    """(t, outer, inner stride), of a contiguous copy if the TMA cannot read t itself."""
+    strides = _tile_strides(t)
+    if strides is None:
+        t = t.clone(memory_format=torch.contiguous_format)
+        strides = t.stride()[:2]
+    return t, *strides
 
 
 def read_prefix_error(device=None, clear=True) -> int:

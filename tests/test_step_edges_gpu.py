@@ -63,3 +63,21 @@ def test_outputs_shared_by_rows_are_refused():
     P.check(one, _attend(one, output=torch.empty((1, 32, 512), dtype=torch.bfloat16, device="cuda").expand(1, 32, 512)), SCALE)
     turned = torch.empty((32, 3, 512), dtype=torch.bfloat16, device="cuda").transpose(0, 1)
     P.check(c, _attend(c, output=turned, lse=torch.empty((32, 3), device="cuda").T), SCALE)
+
+
+def test_refused_caches_are_not_copied():
+    """A cache that the loads cannot read is refused, without a copy of it being made first."""
+    pages = 2000
+    c = P.make_case(3, 2, 16, 100, [1, 70])
+    wide = torch.zeros((pages, 64, 580), dtype=torch.bfloat16, device="cuda")
+    good = torch.zeros((pages, 64, 576), dtype=torch.bfloat16, device="cuda")
+    shifted = torch.zeros(pages * 64 * 512 + 8, dtype=torch.bfloat16, device="cuda")[4:pages * 64 * 512 + 4]
+    _attend(c)
+    for ckv, kpe in ((wide[..., :512], wide[..., 512:576]), (shifted.view(pages, 64, 512), good[..., 512:]),
+                     (good[..., :512], wide[..., 516:])):
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        with pytest.raises(AssertionError, match="cache rows"):
+            _attend(c, ckv=ckv, kpe=kpe)
+        assert torch.cuda.max_memory_allocated() - before < 2 ** 20
