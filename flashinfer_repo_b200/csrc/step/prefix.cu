@@ -115,7 +115,8 @@ struct Deal {
 
 // Tiles of a row block's page list: the prefix, then for every run of tokens of
 // the same request the pages that all of them see whole, once, and for every
-// token the pages that are left.
+// token the pages that are left.  Tokens without own rows (padded rows are of
+// request 0) are of no request here: in a run they would leave it nothing to share.
 __device__ int tiles_of(const PrefixParams& p, int block, int pre_pages) {
   const int t0 = first_token(p, block), nt = tokens_of(p, block);
   int request[kGroups], len[kGroups];  // all loads first: they are in flight together
@@ -128,6 +129,7 @@ __device__ int tiles_of(const PrefixParams& p, int block, int pre_pages) {
 #pragma unroll
   for (int i = 0; i < kGroups; ++i) {
     const int own = own_rows(p, request[i], len[i]);
+    if (own == 0) request[i] = -1;
     if (i > 0 && i < nt && request[i] == request[i - 1]) {
       least = min(least, own);
       ++more;
@@ -339,6 +341,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
       if (bad_rows(p, request, len)) set_error(p.err, kErrBadIndex);
       len = own_rows(p, request, len);
+      if (len == 0) request = -1;  // as in tiles_of
       // groups of the block that are this token's; those behind the last one
       // are nobody's and their lanes may be written
       const int g0 = (t0 + lane) * p.group_per_token - block * kGroups;

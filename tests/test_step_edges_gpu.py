@@ -81,3 +81,35 @@ def test_refused_caches_are_not_copied():
         with pytest.raises(AssertionError, match="cache rows"):
             _attend(c, ckv=ckv, kpe=kpe)
         assert torch.cuda.max_memory_allocated() - before < 2 ** 20
+
+
+@pytest.mark.parametrize("heads,live,padded,own", [(16, 5, 3, 6000), (16, 3, 13, 700), (32, 2, 6, 1000)])
+def test_padded_rows_leave_the_pages_of_a_request_shared(heads, live, padded, own):
+    """One request with several tokens and rows behind the last one (request 0, length 0, as step_layout makes them):
+    its own pages are in the list of the row block once, not once a token."""
+    tokens = live + padded
+    c = P.make_case(4, 1, heads, 200, [own])
+    c["lens"] = _put(*(own - live + 1 + i for i in range(live)), *[0] * padded)
+    c["request"] = torch.zeros(tokens, dtype=I32, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(5)
+    c["qn"] = torch.randn((tokens, heads, 512), generator=g, device="cuda").to(torch.bfloat16)
+    c["qp"] = torch.randn((tokens, heads, 64), generator=g, device="cuda").to(torch.bfloat16)
+    ws = torch.zeros(fi.prefix_workspace_size(tokens, heads), dtype=torch.uint8, device="cuda")
+    got = _attend(c, workspace=ws)
+    P.check(c, got, SCALE)
+    blocks = -(-tokens * (heads // 16) // 8)
+    tiles = ws[256:256 + 8 * (blocks + 1)].view(torch.int64).diff().tolist()
+    # the prefix, the pages that all live tokens see whole, and one more for each token, two pages a tile
+    assert tiles[0] <= (4 + own // 64 + 2 * live + 1) // 2 + 1, tiles
+
+
+def test_empty_rows_between_the_tokens_of_a_request():
+    c = P.make_case(6, 2, 16, 130, [400, 90])
+    c["lens"], c["request"] = _put(300, 0, 399, 400, 0, 0, 90, 0, 77), _put(0, 0, 0, 0, 1, 0, 1, 1, 1)
+    g = torch.Generator(device="cuda").manual_seed(7)
+    c["qn"] = torch.randn((9, 16, 512), generator=g, device="cuda").to(torch.bfloat16)
+    c["qp"] = torch.randn((9, 16, 64), generator=g, device="cuda").to(torch.bfloat16)
+    P.check(c, _attend(c), SCALE)
+    c["prefix"].zero_()
+    P.check(c, _attend(c), SCALE)
+    assert fi.read_prefix_error() == 0
