@@ -60,6 +60,23 @@ def _check_rotation(positions, inv_freq, tokens, layout):
     return positions.contiguous(), inv_freq.contiguous()
 
 
+class _Turn(torch.autograd.Function):
+    """The turn with its gradient, the turn back."""
+
+    @staticmethod
+    def forward(ctx, x, positions, inv_freq, layout, offset, inverse, scale):
+        ctx.save_for_backward(positions, inv_freq)
+        ctx.turn = layout, offset, inverse, scale
+        return apply_rope(x, positions, inv_freq, layout=layout, offset=offset, inverse=inverse, scale=scale)
+
+    @staticmethod
+    def backward(ctx, grad):
+        positions, inv_freq = ctx.saved_tensors
+        layout, offset, inverse, scale = ctx.turn
+        grad = apply_rope(grad, positions, inv_freq, layout=layout, offset=offset, inverse=not inverse, scale=scale)
+        return grad, None, None, None, None, None, None
+
+
 def apply_rope(x, positions, inv_freq, *, layout="interleaved", offset=0, inverse=False, scale=1.0, out=None):
     """Turn the slice [offset, offset + rot_dim) of every head of x [T, H, D]
     (or [T, D]) to its token's position, rot_dim = 2 * len(inv_freq); the other
@@ -69,10 +86,15 @@ def apply_rope(x, positions, inv_freq, *, layout="interleaved", offset=0, invers
     layout "interleaved" pairs values (2i, 2i+1) of the slice, "half" (i, i +
     rot_dim/2).  scale multiplies the turned slice (the attention factor of
     scaled frequencies).  inverse=True turns back: with the same scale it is the
-    gradient of the forward turn.  out: a tensor of x's shape and type to write
-    into, x itself for in place; any other overlap with x is not allowed.
+    gradient of the forward turn, which autograd records for an x that requires
+    one.  out: a tensor of x's shape and type to write into, x itself for in
+    place (nothing can be recorded then); any other overlap with x is not allowed.
     bf16, fp16 or fp32; products in 32 bits, one rounding.
     """
+    if torch.is_grad_enabled() and (x.requires_grad or inv_freq.requires_grad):
+        if out is not None or inv_freq.requires_grad:
+            raise RuntimeError("apply_rope records gradients of x only, and not into out=: use torch.no_grad()")
+        return _Turn.apply(x, positions, inv_freq, layout, offset, inverse, scale)
     shape = x.shape
     assert len(shape) in (2, 3), "x must be [tokens, heads, dim] or [tokens, dim]"
     dtype = DTYPES.get(x.dtype)

@@ -113,3 +113,66 @@ def test_empty_rows_between_the_tokens_of_a_request():
     c["prefix"].zero_()
     P.check(c, _attend(c), SCALE)
     assert fi.read_prefix_error() == 0
+
+
+# ------------------------------------------------------------------ rotary
+def _turn64(x, pos, inv, layout, offset, scale):
+    ang = pos.double()[:, None, None] * inv
+    c, s, r = torch.cos(ang), torch.sin(ang), 2 * inv.numel()
+    z = x[..., offset:offset + r]
+    a, b = (z[..., 0::2], z[..., 1::2]) if layout == "interleaved" else z.chunk(2, -1)
+    y = ((a * c - b * s) * scale, (b * c + a * s) * scale)
+    y = torch.stack(y, -1).flatten(-2) if layout == "interleaved" else torch.cat(y, -1)
+    return torch.cat((x[..., :offset], y, x[..., offset + r:]), -1)
+
+
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+@pytest.mark.parametrize("flat", [False, True])
+def test_rope_gradient_follows_the_result(layout, flat):
+    """A tensor that requires gradients gets the formula's, through a strided view and a second time over."""
+    g = torch.Generator(device="cuda").manual_seed(8)
+    leaf = torch.randn((9, 5, 104), generator=g, device="cuda", requires_grad=True)
+    pos, inv = torch.arange(9, device="cuda", dtype=I32) * 7919, fi.rope_frequencies(64)
+    dy = torch.randn((9, 5, 96), generator=g, device="cuda")
+    view = leaf[..., 8:]
+    if flat:
+        view, dy = view[:, 2], dy[:, 2].contiguous()
+    y = fi.apply_rope(view, pos, inv, layout=layout, offset=16, scale=1.3)
+    (grad,) = torch.autograd.grad(y, leaf, dy, create_graph=False)
+    l64 = leaf.detach().double().requires_grad_()
+    v64 = l64[..., 8:]
+    ref = _turn64(v64[:, 2][:, None] if flat else v64, pos, inv, layout, 16, 1.3)
+    (want,) = torch.autograd.grad(ref, l64, (dy[:, None] if flat else dy).double())
+    # |a| + |b| of two normal values stays below 12, scaled by 1.3; 7e-7 of it: the angle's rounding and the products
+    assert (grad.double() - want).abs().max() <= 1.3 * 12 * 7e-7 + 12 * 2 ** -24
+    assert (y.detach().double() - (ref[:, 0] if flat else ref)).abs().max() <= 1.3 * 12 * 7e-7 + 12 * 2 ** -24
+    # against differences: the turn is linear, so they are exact up to rounding
+    step = torch.randn(leaf.shape, generator=g, device="cuda")
+    with torch.no_grad():
+        moved = (leaf + step)[..., 8:]
+        moved = fi.apply_rope(moved[:, 2] if flat else moved, pos, inv, layout=layout, offset=16, scale=1.3)
+        slope, along = ((moved - y) * dy).double().sum(), (grad * step).double().sum()
+    n = dy.numel()
+    assert (slope - along).abs() <= n ** 0.5 * 8 * 12 * 12 * 1e-6
+
+
+def test_rope_gradient_is_recorded_only_where_wanted():
+    x = torch.randn((4, 2, 64), device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    pos, inv = _put(1, 2, 3, 4), fi.rope_frequencies(64)
+    y = fi.apply_rope(x, pos, inv)
+    assert y.requires_grad and y.dtype == torch.bfloat16
+    with torch.no_grad():
+        z = fi.apply_rope(x, pos, inv)
+        fi.apply_rope(x, pos, inv, out=x)  # in place is fine where nothing is recorded
+    assert not z.requires_grad and torch.equal(y, z) and torch.equal(x, z)
+    assert not fi.apply_rope(x.detach(), pos, inv).requires_grad
+    for out in (x, torch.empty_like(x)):
+        with pytest.raises(RuntimeError, match="grad"):
+            fi.apply_rope(x, pos, inv, out=out)
+    with pytest.raises(RuntimeError, match="grad"):
+        fi.apply_rope(x.detach(), pos, inv.clone().requires_grad_())
+    # twice differentiable: the turn of the turned-back gradient
+    dy = torch.randn((4, 2, 64), device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    (g,) = torch.autograd.grad(fi.apply_rope(x, pos, inv), x, dy, create_graph=True)
+    (h,) = torch.autograd.grad(g, dy, torch.ones_like(g))
+    assert torch.equal(h, fi.apply_rope(torch.ones_like(x), pos, inv).detach())
