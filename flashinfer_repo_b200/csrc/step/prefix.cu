@@ -1152,9 +1152,13 @@ extern "C" int dsa_shared_prefix_attention_scratch(
   if (e == cudaSuccess && pairs > 1 && !whole) {
     const int rows = (p.groups < kGroups ? p.groups : kGroups) * 16, by_cut = p.blocks >= pairs;
     const unsigned x = rows / kMergeRows, y = (unsigned)(by_cut ? pairs - 1 : p.blocks), threads = kMergeRows * kMergeColumns;
-    // few row blocks have many partials each: more of them in flight, and over 16
-    // dealt out to 8 threads (a token behind 131072 rows, 74 partials: 56 -> 42 us a call)
-    if (pairs / p.blocks > 16)
+    // few row blocks have many partials each: more of them in flight, and over 24
+    // dealt out to 8 threads.  With one, two, three, four row blocks of 128 rows
+    // behind 20000 rows (74 to 18 partials) 8 threads take 19.7, 23.7, 29.0, 33.1 us
+    // a call, one thread 25.6, 24.2, 26.9, 29.3.  One thread with 10 partials in
+    // flight against four column quads a thread with 2: 16 row blocks of 4 partials
+    // 74.4 against 71.8 us, 5 of 14 34.9 against 39.1.
+    if (pairs / p.blocks > 24)
       e = launch_after(dsa_prefix_merge_kernel<1, 5, 8>, dim3(32 * x, y), threads, 0, s, p, by_cut);
     else if (x * y <= 148)
       e = launch_after(dsa_prefix_merge_kernel<1, 10, 1>, dim3(4 * x, y), threads, 0, s, p, by_cut);
