@@ -84,7 +84,8 @@ def build_probes(force: bool = False) -> list:
     outs = []
     for src in sorted(glob.glob(os.path.join(PROBES, "*.cu"))):
         exe = src[:-3]
-        if force or _stale(exe, [src] + glob.glob(os.path.join(CSRC, "*.cuh"))):
+        if force or _stale(exe, [src] + glob.glob(os.path.join(CSRC, "*.cuh")) +
+                           glob.glob(os.path.join(CSRC, "step", "*.cuh"))):
             subprocess.check_call([nvcc()] + NVCC_FLAGS + ["-o", exe, src, "-lcuda"])
         outs.append(exe)
     return outs
