@@ -4,9 +4,11 @@
 // Sums and products in 32 bits, one rounding at the store.
 //
 // One warp per row: 16 latent values and one rotary pair a lane, the sum of
-// squares by shuffles, one angle a lane.  Bound by HBM for a prefill batch
-// (1152 bytes in and out a row; 16384 rows 6.8 us, 85% of the copy rate) and by
-// latency for a decode step (64 rows 2.0 us).
+// squares by shuffles, one angle a lane.  1152 bytes in and out a row: 16384 rows,
+// 38 MB, take 6.8 us where inputs and cache are in L2, as behind the projection
+// that made them, and 9.8 us from HBM (12 sets of them in turn): 3.9 TB/s, 59% of
+// the copy rate.  That grid is over after three rounds of CTAs, so the first loads
+// and the last round weigh.  A decode step is latency (64 rows 1.7-2.0 us).
 #include "../../../include/dsa_b200.h"
 #include "rotate.cuh"
 
@@ -32,7 +34,10 @@ struct AppendParams {
 };
 
 // 8 values from `from` on as they are wanted in the sum: 32 bits.  kOnce: nobody
-// reads them again (first to leave L2: 16384 rows 10.1 -> 9.1 us from cold).
+// reads them again, so they leave L2 first and push out less that has to be written
+// back: 16384 rows behind 512 MB of other writes 12.3 instead of 14.3 us (timed by
+// events around the call); 2-4% slower where L2 holds all or nothing of them (6.8
+// against 6.5 us, 9.8 against 9.6).
 template <typename T, bool kVec, bool kOnce>
 __device__ __forceinline__ void load8(const T* from, float* v) {
   if (kVec) {
@@ -50,8 +55,8 @@ __device__ __forceinline__ void load8(const T* from, float* v) {
   }
 }
 
-// 4 rows a CTA: with 8 a decode step took 1.97 instead of 1.78 us, 16384 rows 9.1
-// instead of 8.2.
+// 4 rows a CTA: with 8 a decode step takes 1.88 instead of 1.70 us, 16384 rows 7.15
+// instead of 6.8 (from L2) and 10.7 instead of 9.8.
 constexpr int kAppendThreads = 128;
 
 template <typename T, typename W, bool kVec>

@@ -25,7 +25,7 @@ namespace dsa {
 namespace {
 
 // Small CTAs: the scan's depth is what a call waits for (64 requests / 32768 rows of
-// 509: 3.0 / 3.8 us; with 512 threads 3.9 / 4.7, with 8 requests a thread 3.5 / 4.5).
+// 509: 3.0 / 3.7 us; with 512 threads 3.6 / 4.4, with 8 requests a thread 3.5 / 4.4).
 constexpr int kLayThreads = 128;
 constexpr int kLayItems = 4;                         // requests per thread and chunk
 constexpr int kLayChunk = kLayThreads * kLayItems;

@@ -24,10 +24,11 @@
 // filled page is loaded from a row coordinate below zero, which moves its rows to
 // the end of the tile and has the TMA write zeros before them.
 //
-// Bound by the MMA: 2186 cycles a tile alone, 2510-2800 here.  128 tokens of 128
-// heads behind 16384 rows: 458 us, 1.29 PFLOP/s at the clock that the power limit
-// leaves (94% of what a cuBLAS product sustains); 64 tokens of 16 heads behind
-// 32768 rows: 64-79 us, 20 of them the plan, the first loads, partials and merge.
+// Bound by the MMA: 2196 cycles a tile alone (36 at N = 128 of 32.4, 16 at N = 256
+// of 64.4), 2510-2800 here.  128 tokens of 128 heads behind 16384 rows: 440-470 us,
+// 1.25-1.34 PFLOP/s at the clock that the power limit leaves (91% or more of what a
+// cuBLAS product sustains); 64 tokens of 16 heads behind 32768 rows: 66-80 us, 20 of
+// them the plan, the first loads, partials and merge.
 #include <cuda.h>
 
 #include <mutex>
@@ -48,7 +49,11 @@ constexpr int kSoftmaxThreads = 256;
 constexpr uint32_t kTmemS = 256;               // TMEM columns: O 0-255, scores 256 and 320
 constexpr int kSlotFloats = 2 * kRows * 512 + 4 * kRows;  // partial: O, m, l of 128 rows
 constexpr int kCutTiles = 3;  // what a second row block costs a pair: queries, a refill and a partial, in tiles
-constexpr int kL2Pages = 1300;  // pages of 73728 bytes that stay in the 126 MB of L2 beside the rest
+// Pages of 73728 bytes that stay in the 126 MB of L2 beside the rest: where row blocks
+// walk the prefix in step or not makes no difference up to 80000 rows (141.8 and 141.7
+// us for 8 tokens of 128 heads); beyond, in step is sooner done (90000 rows 156 against
+// 165 us, 131072 218 against 234, 180000 297 against 331).
+constexpr int kL2Pages = 1300;
 constexpr int kSoloBlocks = 64;  // row blocks that a warp plans alone: 2 a lane
 constexpr int kWholeTiles = 3;
 constexpr float kLazy = 8.f;  // the running maximum follows only a rise of more than 2^8
@@ -695,7 +700,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         uint32_t w[16];
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-          // weights are rounded to bf16 for the matrix product, the sum takes them as they are
+          // Weights are rounded to bf16 for the matrix product, whose two operands are of
+          // one type (in two parts they would cost 47% more MMA); the sum takes them as
+          // they are.  Each is off by at most 2^-8 of itself, independently of the others:
+          // a bf16 output's error against 64 bits grows from 1.7e-3 of its norm, the
+          // output's own rounding, to 1.7e-3 (32768 rows) - 2.1e-3 (1000 rows).
           float2 e = fma2(x[j], make_float2(p.scale_log2, p.scale_log2), make_float2(sub, sub));
           e = make_float2(ex2_approx(e.x), ex2_approx(e.y));
           sums = add2(sums, e);
@@ -1092,9 +1101,10 @@ extern "C" int dsa_shared_prefix_attention_scratch(
     return report_error(DSA_ERR_WORKSPACE, "workspace too small or not 256-byte aligned");
   // What the host knows of the work: the longest list a row block can have.  No
   // more pairs than tiles are launched, and up to kWholeTiles tiles are left to
-  // one pair a row block: on the GPU as soon done as a split and its merge grid
-  // (a token behind 200 rows: 11.7 against 11.3 us), and one launch less for the
-  // host (20 against 22 us a call).
+  // one pair a row block: one launch less for the host (20 against 22 us a call),
+  // and on the GPU as soon done as a split and its merge grid.  Two tiles 11.5 us
+  // either way for a token, 12.7 against 14.6 for 16 row blocks; three 12.9 against
+  // 11.5 and 14.3 against 15.8; four 11.5 for the split against 14.2 whole.
   const int64_t per = num_heads / 16;  // 16-head groups of a token
   const int64_t block_tokens = kGroups % per == 0 ? kGroups / per : per % kGroups == 0 ? 1 : (kGroups + per - 1) / per + 1;
   const int64_t block_pages = (max_prefix_len + 63) / 64 + (block_tokens < num_tokens ? block_tokens : num_tokens) * max_pages;
